@@ -19,6 +19,7 @@ FL_MAX_RANK = 8
 
 # enum fl_dtype (numbering of the reference's ``enum class Type``, include/utils/type.h:11-19)
 FL_UNKNOWN, FL_BOOL, FL_INT32, FL_INT64, FL_FLOAT16, FL_FLOAT32, FL_FLOAT64 = range(7)
+FL_BFLOAT16 = 16
 
 # enum fl_ref_flags
 FL_REF_CONV_UNIT_STRIDE = 1 << 0
@@ -36,7 +37,11 @@ FL_ERR_UNSUPPORTED = -8
 FL_ERR_STATIC_SCRATCH = -9
 FL_NO_ALLOC_SCRATCH_BYTES = 2 << 20
 
-DTYPE_SIZE = {FL_BOOL: 1, FL_INT32: 4, FL_INT64: 8, FL_FLOAT16: 2, FL_FLOAT32: 4, FL_FLOAT64: 8}
+DTYPE_SIZE = {FL_BOOL: 1, FL_INT32: 4, FL_INT64: 8, FL_FLOAT16: 2, FL_FLOAT32: 4, FL_FLOAT64: 8, FL_BFLOAT16: 2}
+
+# enum fl_rotary_scaling, enum fl_gate_activation
+FL_ROTARY_PLAIN, FL_ROTARY_LINEAR, FL_ROTARY_BASE, FL_ROTARY_WAVELENGTH, FL_ROTARY_DIMENSION = range(5)
+FL_GATE_SILU, FL_GATE_GELU, FL_GATE_GELU_TANH, FL_GATE_RELU, FL_GATE_SIGMOID, FL_GATE_IDENTITY = range(6)
 
 
 class FlTensor(ctypes.Structure):
@@ -190,6 +195,13 @@ SIGNATURES = {
     "fluidml_hip_add_layer_normalization": [_T, _T, _T, _T, _T, _i64, _f64, _vp],
     "fluidml_hip_gather_constant_data_tensor_stats": [_T, _T, _T, _vp, _vp],
     "fluidml_hip_gather_add_layer_normalization": [_T, _T, _T, _T, _T, _T, _T, _T, _f64, _vp],
+    # decoder operators
+    "fluidml_hip_rotary_positions": [_T, _T, _T, _vp, _vp],
+    "fluidml_hip_rotary_positions_pair": [_T, _T, _T, _T, _T, _vp, _vp],
+    "fluidml_hip_attention_positions_scratch": [_T, _T, _vp, _P(_sz)],
+    "fluidml_hip_attention_positions": [_T, _T, _T, _T, _vp, _vp, _sz, _vp],
+    "fluidml_hip_gated_matmul": [_T, _T, _T, _T, _T, _T, _i32, _vp],
+    "fluidml_hip_gated_feed_forward": [_T, _T, _T, _T, _T, _T, _T, _T, _T, _T, _i32, _vp],
     "fluidml_hip_conv_without_padding": [_T, _T, _T, _T, _i64p, _i64p, _i64, _u32, _vp],
     "fluidml_hip_conv_with_padding": [_T, _T, _T, _T, _vp, _sz, _i64p, _i64p, _i64p, _i64, _u32, _vp],
 }
@@ -216,6 +228,20 @@ class FlNormFusion(ctypes.Structure):
     _fields_ = [("deferred", ctypes.c_int32), ("width", ctypes.c_int32), ("epsilon", ctypes.c_double),
                 ("stats", ctypes.c_void_p), ("scale", ctypes.POINTER(FlTensor)), ("shift", ctypes.POINTER(FlTensor)),
                 ("stats_out", ctypes.c_void_p), ("addend2", ctypes.POINTER(FlTensor))]
+
+
+class FlRotaryPlan(ctypes.Structure):
+    """fl_rotary_plan of include/fluidml_hip.h"""
+    _fields_ = [("interleaved", ctypes.c_int32), ("scaling", ctypes.c_int32), ("dims", ctypes.c_int64), ("base", ctypes.c_double),
+                ("factor", ctypes.c_double), ("original_length", ctypes.c_double), ("low", ctypes.c_double),
+                ("high", ctypes.c_double), ("amplitude", ctypes.c_double)]
+
+
+class FlAttentionScores(ctypes.Structure):
+    """fl_attention_scores of include/fluidml_hip.h"""
+    _fields_ = [("scale", ctypes.c_double), ("cap", ctypes.c_double), ("slopes", _T), ("causal", ctypes.c_int32),
+                ("window", ctypes.c_int64), ("prefix_lengths", _T), ("query_documents", _T), ("key_documents", _T),
+                ("query_starts", _T), ("query_lengths", _T), ("key_lengths", _T)]
 
 
 FL_NORM_NONE, FL_NORM_LHS, FL_NORM_ADDEND = 0, 1, 2
@@ -286,6 +312,18 @@ def make_tensor(base: int, dtype: int, shape: Sequence[int], strides: Optional[S
         t.shape[i] = int(s)
         t.strides[i] = int(st)
     return t
+
+
+_TORCH_DTYPES = {"torch.bool": FL_BOOL, "torch.int32": FL_INT32, "torch.int64": FL_INT64, "torch.float16": FL_FLOAT16,
+                 "torch.bfloat16": FL_BFLOAT16, "torch.float32": FL_FLOAT32, "torch.float64": FL_FLOAT64}
+
+
+def view(t) -> FlTensor:
+    """The view that a torch tensor is: its address, type, shape and strides (the tensor has to outlive its uses)."""
+    rank = t.dim()
+    if rank > FL_MAX_RANK:
+        raise ValueError(f"rank {rank} exceeds FL_MAX_RANK={FL_MAX_RANK}")
+    return FlTensor(t.data_ptr(), _TORCH_DTYPES[str(t.dtype)], rank, tuple(t.shape), t.stride())
 
 
 def i64_array(values: Iterable[int]):

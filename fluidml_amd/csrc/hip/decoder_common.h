@@ -1,0 +1,58 @@
+// Shared by the decoder operators (rotary.hip, attention_positions.hip, gated.hip): views that may reach beyond 2^31 elements and the three types
+// they compute on.
+#ifndef FLUIDML_AMD_CSRC_HIP_DECODER_COMMON_H_
+#define FLUIDML_AMD_CSRC_HIP_DECODER_COMMON_H_
+
+#include "fl_common.h"
+
+namespace fl {
+
+inline bool IsDecoderType(int32_t dtype) { return dtype == FL_FLOAT32 || dtype == FL_FLOAT16 || dtype == FL_BFLOAT16; }
+
+// CheckView for these operators: 64-bit offsets, FL_BFLOAT16 among the types
+inline int CheckWideView(const fl_tensor *t) {
+  if (t == nullptr || t->base == nullptr) return FL_ERR_NULL;
+  if (t->rank < 0 || t->rank > kMaxRank) return FL_ERR_RANK;
+  if (DtypeSize(t->dtype) == 0 && t->dtype != FL_BFLOAT16) return FL_ERR_DTYPE;
+  __int128 span = 0;
+  for (int i = 0; i < t->rank; ++i) {
+    if (t->shape[i] <= 0 || t->strides[i] < 0) return FL_ERR_SHAPE;
+    if (t->shape[i] > FL_DECODER_MAX_EXTENT) return FL_ERR_TOO_LARGE;
+    span += static_cast<__int128>(t->shape[i] - 1) * t->strides[i];
+    if (span > (static_cast<__int128>(1) << 48)) return FL_ERR_TOO_LARGE;
+  }
+  return FL_OK;
+}
+
+// ... of a result: no two elements in one place along a dim
+inline int CheckWideResult(const fl_tensor *t) {
+  FL_CHECK(CheckWideView(t));
+  for (int i = 0; i < t->rank; ++i) {
+    if (t->shape[i] > 1 && t->strides[i] == 0) return FL_ERR_SHAPE;
+  }
+  return FL_OK;
+}
+
+// [n] of type `dtype`, or [n] that is NULL
+inline int CheckOptionalVector(const fl_tensor *t, int32_t dtype, int64_t n) {
+  if (t == nullptr) return FL_OK;
+  FL_CHECK(CheckWideView(t));
+  if (t->rank != 1) return FL_ERR_RANK;
+  if (t->dtype != dtype) return FL_ERR_DTYPE;
+  return t->shape[0] == n ? FL_OK : FL_ERR_SHAPE;
+}
+
+// body(a value of the C++ type of `dtype`)
+template <typename F>
+inline int ForDecoderType(int32_t dtype, F &&body) {
+  switch (dtype) {
+    case FL_FLOAT32: return body(float{});
+    case FL_FLOAT16: return body(static_cast<_Float16>(0));
+    case FL_BFLOAT16: return body(static_cast<__bf16>(0.0f));
+    default: return FL_ERR_DTYPE;
+  }
+}
+
+}  // namespace fl
+
+#endif  // FLUIDML_AMD_CSRC_HIP_DECODER_COMMON_H_

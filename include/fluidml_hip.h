@@ -46,9 +46,10 @@ enum fl_dtype {
   FL_BOOL = 1, /* 1 byte, values 0/1 (sizeof(bool), reference src/utils/type.cpp:45) */
   FL_INT32 = 2,
   FL_INT64 = 3,
-  FL_FLOAT16 = 4, /* carried, never computed on */
+  FL_FLOAT16 = 4, /* carried, never computed on but by the decoder operators */
   FL_FLOAT32 = 5,
-  FL_FLOAT64 = 6
+  FL_FLOAT64 = 6,
+  FL_BFLOAT16 = 16 /* no type of the reference: the decoder operators below compute on it, and on FL_FLOAT16 */
 };
 
 enum fl_error {
@@ -615,6 +616,95 @@ int fluidml_hip_gather_add_layer_normalization(const fl_tensor *indices0, const 
  * out = LayerNorm(lhs + rhs) (reference add.cpp:75-137 +
  * layer_normalization.cpp:33-220, ONNX semantics). */
 int fluidml_hip_add_layer_normalization(const fl_tensor *lhs, const fl_tensor *rhs, const fl_tensor *scale, const fl_tensor *bias, const fl_tensor *out, int64_t axis, double epsilon, void *stream);
+
+/* ------------------------------------------------------------------------- */
+/* Decoder operators: what layers of newer decoders need beside the kernels    */
+/* above (no counterpart in the reference).  Operands are FL_FLOAT32,          */
+/* FL_FLOAT16 or FL_BFLOAT16, all of one type; sums, softmax statistics and    */
+/* angles are held in 32 bits or more and results rounded once.  Views may     */
+/* reach beyond 2^31 elements; every extent is at least 1 and at most          */
+/* FL_DECODER_MAX_EXTENT, strides are not negative, and a result does not      */
+/* overlap an operand or itself but where a call says so.  Operands live on    */
+/* the current device, which is the stream's.  The calls allocate nothing,     */
+/* synchronise nothing and may be captured; two calls that may run at the same */
+/* time (a replayed graph among them) need scratch and results of their own.   */
+#define FL_DECODER_MAX_EXTENT (1 << 28)
+
+/* Rotary positions.  The pair j < dims / 2 of columns (a, b) of a token at position p becomes
+ *   (a c - b s, b c + a s),  c = amplitude cos(p f_j), s = amplitude sin(p f_j);
+ * columns from `dims` on are copied.  Pairs are columns (j, j + dims / 2), with `interleaved` (2 j, 2 j + 1).
+ * f_j = base^(-2 j / dims), for contexts longer than the trained one changed as `scaling` says:
+ *   FL_ROTARY_LINEAR      f_j / factor
+ *   FL_ROTARY_BASE        base * factor^(dims / (dims - 2)) in place of base: the shortest wave stays, the longest is stretched by `factor`
+ *   FL_ROTARY_WAVELENGTH  t = original_length f_j / 2 pi turns within the trained length: kept from `high` turns on, divided by
+ *                         `factor` up to `low`, and mixed between: f_j (m + (1 - m) / factor), m = (t - low) / (high - low)
+ *   FL_ROTARY_DIMENSION   the same mix with a ramp over j: d(t) = dims ln(original_length / 2 pi t) / (2 ln base) is the j whose
+ *                         wave turns t times; kept up to max(0, floor(d(high))), divided from min(dims - 1, ceil(d(low))) on
+ * Angles are computed in 64 bits, so that far positions lose nothing. */
+enum fl_rotary_scaling { FL_ROTARY_PLAIN = 0, FL_ROTARY_LINEAR = 1, FL_ROTARY_BASE = 2, FL_ROTARY_WAVELENGTH = 3, FL_ROTARY_DIMENSION = 4 };
+#define FL_ROTARY_MAX_DIMS 1024
+typedef struct fl_rotary_plan {
+  int32_t interleaved; /* 0 or 1 */
+  int32_t scaling;     /* enum fl_rotary_scaling */
+  int64_t dims;        /* even, 2 .. min(D, FL_ROTARY_MAX_DIMS) */
+  double base;         /* > 1 */
+  double factor;       /* >= 1; what a scaling does not use is not looked at */
+  double original_length; /* > 0 */
+  double low, high;       /* 0 < low < high */
+  double amplitude;       /* finite; 1 where nothing else is wanted */
+} fl_rotary_plan;
+/* x, out [B, H, S, D], any strides; `out` may be `x` itself.  positions: int32 or int64, [S], [1, S] or [B, S], of either sign. */
+int fluidml_hip_rotary_positions(const fl_tensor *x, const fl_tensor *positions, const fl_tensor *out, const fl_rotary_plan *plan, void *stream);
+/* The same for two tensors of one B, S, D and type at the same positions in ONE launch (queries and keys; the heads may differ). */
+int fluidml_hip_rotary_positions_pair(const fl_tensor *x0, const fl_tensor *out0, const fl_tensor *x1, const fl_tensor *out1, const fl_tensor *positions, const fl_rotary_plan *plan, void *stream);
+
+/* Attention whose scores and masks go by positions, so that no mask is read and keys that no query of a tile sees cost
+ * nothing:
+ *   s_ij = scale (q_i . k_j);  cap > 0: s_ij = cap tanh(s_ij / cap);  slopes: s_ij -= slopes[h] |p_i - j|
+ *   out_i = sum_j softmax_j(s_ij) v_j over the keys that query i sees; zeros where it sees none
+ * q, out [B, H, Sq, D], k, v [B, KV, Skv, D], any strides; head h reads key head h / (H / KV) (H a multiple of KV); D <=
+ * FL_ATTENTION_MAX_HEAD.  Key j of a sequence is at position j, query i at p_i = query_starts[b] + i, without query_starts
+ * at key_lengths[b] - query_lengths[b] + i (the last query at the last key).  Query i sees key j where all of these hold:
+ *   j < key_lengths[b] (without them: Skv);
+ *   the documents of i and j are equal and not negative, where documents are given (a negative one marks padding);
+ *   j < prefix_lengths[b], or both: not causal, or j <= p_i; no window, or p_i - window < j < p_i + window.
+ * Rows i >= query_lengths[b] of out are left as they were.  What a query does not see does not reach it, whatever it holds
+ * (infinities and NaN too).  Lengths are clamped to 0 .. Skv or Sq.  With 16-bit operands the softmax's weights are rounded
+ * to that type before the product with v, as v itself is. */
+#define FL_ATTENTION_MAX_HEAD 256
+typedef struct fl_attention_scores {
+  double scale;
+  double cap;              /* 0: none */
+  const fl_tensor *slopes; /* float32 [H]; NULL: none (as all that follow) */
+  int32_t causal;          /* 0 or 1 */
+  int64_t window;          /* 0: none */
+  const fl_tensor *prefix_lengths;  /* int32 [B] */
+  const fl_tensor *query_documents; /* int32 [B, Sq], with key_documents [B, Skv]: both or none */
+  const fl_tensor *key_documents;
+  const fl_tensor *query_starts;  /* int32 [B] */
+  const fl_tensor *query_lengths; /* int32 [B] */
+  const fl_tensor *key_lengths;   /* int32 [B] */
+} fl_attention_scores;
+/* `scratch`: at least as many bytes as ..._scratch says for these operands (which may be none), 16-byte aligned, of any contents; in use until the
+ * call's work is done. */
+int fluidml_hip_attention_positions_scratch(const fl_tensor *q, const fl_tensor *k, const fl_attention_scores *scores, size_t *bytes);
+int fluidml_hip_attention_positions(const fl_tensor *q, const fl_tensor *k, const fl_tensor *v, const fl_tensor *out, const fl_attention_scores *scores, void *scratch, size_t scratch_bytes, void *stream);
+
+/* Gated feed-forward block: products = activation(x . gate + gate_bias) * (x . up + up_bias), both contractions, the activation
+ * and the product in one launch; x [M, K], gate, up [K, N] (any strides; rows of a checkpoint's [N, K] are its transposed view,
+ * two halves of one tensor two views), biases [N] or NULL, products [M, N]. */
+enum fl_gate_activation {
+  FL_GATE_SILU = 0,      /* a / (1 + exp(-a)) */
+  FL_GATE_GELU = 1,      /* a / 2 (1 + erf(a / sqrt 2)) */
+  FL_GATE_GELU_TANH = 2, /* a / 2 (1 + tanh(sqrt(2 / pi) (a + 0.044715 a^3))) */
+  FL_GATE_RELU = 3,
+  FL_GATE_SIGMOID = 4,
+  FL_GATE_IDENTITY = 5
+};
+int fluidml_hip_gated_matmul(const fl_tensor *x, const fl_tensor *gate, const fl_tensor *up, const fl_tensor *gate_bias, const fl_tensor *up_bias, const fl_tensor *products, int32_t activation, void *stream);
+/* The same with the projection behind it: out = products . down + down_bias + addend; down [N, O], down_bias [O] or NULL, addend
+ * [M, O] or NULL (may be `out` itself), out [M, O].  `products` is written, rounded to the operands' type, and read again. */
+int fluidml_hip_gated_feed_forward(const fl_tensor *x, const fl_tensor *gate, const fl_tensor *up, const fl_tensor *gate_bias, const fl_tensor *up_bias, const fl_tensor *down, const fl_tensor *down_bias, const fl_tensor *addend, const fl_tensor *products, const fl_tensor *out, int32_t activation, void *stream);
 
 #ifdef __cplusplus
 }
