@@ -53,6 +53,16 @@ inline int ForDecoderType(int32_t dtype, F &&body) {
   }
 }
 
+#if defined(__HIPCC__)
+// 16 bytes from a lane's own address to 16 * lane bytes behind `to` (the same for all lanes, in LDS), without a register between.
+// Not waited for by the compiler: s_waitcnt vmcnt.  (In the host pass the builtin makes a template kernel lose its launch stub.)
+__device__ __forceinline__ void LoadToLds(const void *from, void *to) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+#endif
+}
+#endif
+
 }  // namespace fl
 
 #endif  // FLUIDML_AMD_CSRC_HIP_DECODER_COMMON_H_

@@ -35,6 +35,20 @@ def attention(q, k, v, scale, cap=0.0, slopes=None, **masks):
     seen, distance, written = visible(B, Sq, Skv, **masks)
     q, k, v = (t.double().cpu() for t in (q, k, v))
     out, most = torch.zeros(B, H, Sq, D, dtype=torch.float64), torch.zeros(B, H, Sq, dtype=torch.float64)
+    if q.isfinite().all() and k.isfinite().all() and v.isfinite().all():  # whole heads at a time: the hidden weights are zeros
+        for b in range(B):
+            for h in range(H):
+                kk, vv = k[b, h // (H // KV)], v[b, h // (H // KV)]
+                s = q[b, h] @ kk.t() * scale
+                if cap:
+                    s = cap * torch.tanh(s / cap)
+                if slopes is not None:
+                    s = s - slopes[h].double().cpu() * distance[b]
+                some = seen[b].any(1, keepdim=True)
+                weights = torch.softmax(s.masked_fill(~seen[b], -math.inf), 1).masked_fill(~some, 0.0)
+                out[b, h] = weights @ vv
+                most[b, h] = torch.where(seen[b], vv.abs().amax(1)[None, :], torch.zeros(())).amax(1)
+        return out, most, written
     for b in range(B):
         for h in range(H):
             kk, vv = k[b, h // (H // KV)], v[b, h // (H // KV)]
@@ -60,7 +74,7 @@ def attention_bound(want, most, dtype, D, Skv, scale, cap, reach, peak=1.0):
     to m) and so is the result; fp16 has steps of 2^-24 where it is denormal, for each of Skv weights (the largest is 1 or more) and the result."""
     import torch
 
-    size = D * scale * peak * peak
+    size = D * abs(scale) * peak * peak
     e = 2.0 ** -24 * (size * (D / 4 + 8) + 8 * (min(cap, size) if cap else 0.0) + (8 * cap if cap else 0) + 4 * reach)
     off = most[..., None] * (2 * e + 2.0 ** -24 * (Skv / 16 + 24))
     if dtype != torch.float32:

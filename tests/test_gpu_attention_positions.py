@@ -121,6 +121,82 @@ def test_attention_positions_sizes(device, dtype, B, H, KV, Sq, Skv, D):
     check(q, k, v, out, 0.3, causal=True)
 
 
+def kernels(q, k, v, out, scale, **more):
+    """Names of what a call launches."""
+    from tests.util import launches
+
+    scratch = oracle.call_attention(q, k, v, out, scale, **more)
+    return [name for name, _ in launches(lambda stream: oracle.call_attention(q, k, v, out, scale, **more, stream=stream, scratch=scratch))]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("name", ALL)
+@pytest.mark.parametrize("B,H,KV,Sq,Skv,D", [
+    (6, 16, 8, 250, 250, 64),      # 500 rows to a key head, the last tile of rows not full
+    (7, 12, 12, 300, 389, 128),    # key heads that do not spread evenly over eight
+    (5, 9, 3, 1200, 330, 72),      # more queries than keys; columns that no sixteen divides
+    (8, 8, 8, 270, 300, 256),
+], ids=["grouped", "cached", "long", "wide"])
+def test_attention_positions_many_rows(device, dtype, name, B, H, KV, Sq, Skv, D):
+    import torch
+
+    print("[case]", dtype, name, B, H, KV, Sq, Skv, D, flush=True)
+    q, k, v = draw(device, dtype_of(dtype), (B, Sq, H, D), (B, Skv, KV, D), (B, Skv, KV, D))
+    q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+    more = options(name, device, B, H, Sq, Skv)
+    out = torch.full_like(q, 7.0)
+    assert any("AttentionRowsKernel" in n for n in kernels(q, k, v, out, D ** -0.5, **more))
+    out.fill_(7.0)
+    oracle.call_attention(q, k, v, out, D ** -0.5, **more)
+    got, written = check(q, k, v, out, D ** -0.5, **more)
+    assert (got[~written[:, None, :].expand(got.shape[:3])] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("name", ["causal", "window", "documents", "prefix", "lengths"])
+def test_attention_positions_many_rows_hidden_values(device, dtype, name):
+    """The same with infinities and NaN in keys that no query sees and in values that some do not see."""
+    import torch
+
+    B, H, KV, Sq, D = 12, 8, 8, 280, 64
+    q, k, v = draw(device, dtype_of(dtype), (B, H, Sq, D), (B, KV, Sq, D), (B, KV, Sq, D))
+    more = options(name, device, B, H, Sq, Sq)
+    if name == "window":
+        more["window"] = 20
+    seen, _, _ = oracle.visible(B, Sq, Sq, **{a: b for a, b in more.items() if a not in ("cap", "slopes")})
+    for b in range(B):
+        k[b, :, ~seen[b].any(0)], v[b, :, ~seen[b].any(0)] = float("nan"), float("inf")
+    some = (seen[3].any(0) & ~seen[3].all(0)).nonzero().flatten()
+    if len(some):
+        v[3, 0, int(some[-1]), 5], v[3, 1, int(some[0]), 7], k[3, 2, int(some[-1]), 9] = float("nan"), float("inf"), float("nan")
+    out = torch.full_like(q, 7.0)
+    assert any("AttentionRowsKernel" in n for n in kernels(q, k, v, out, D ** -0.5, **more))
+    pick = [0, 3, 5]  # (the definition's way takes its time: three sequences of the batch, three heads)
+    more = {a: tuple(t[pick] for t in b) if a == "documents" else b[pick] if hasattr(b, "shape") and a != "slopes" else b for a, b in more.items()}
+    q, k, v, out = (t[pick][:, :3] for t in (q, k, v, out))
+    want, most, _ = oracle.attention(q, k, v, D ** -0.5, **more)
+    got = out.double().cpu()
+    assert torch.equal(got.isnan(), want.isnan())
+    fine = want.isfinite()
+    assert torch.equal(got[~fine & ~want.isnan()], want[~fine & ~want.isnan()])
+    bound = oracle.attention_bound(want, torch.ones_like(most), q.dtype, D, Sq, D ** -0.5, more.get("cap", 0.0), 0.0)
+    assert ((got - want).abs() <= bound)[fine].all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_attention_positions_many_rows_far_scores(device, dtype):
+    import torch
+
+    for order in (1, -1):
+        q, k, v = draw(device, dtype_of(dtype), (3, 8, 1100, 64), (3, 8, 300, 64), (3, 8, 300, 64))
+        ramp = torch.arange(300, device=device).to(torch.float32) / 300
+        ramp = ramp if order == 1 else ramp.flip(0)
+        k = (k * 0.1 + ramp[:, None] * torch.sign(q[:, :, :1].float())).to(q.dtype)
+        out = torch.full_like(q, 7.0)
+        oracle.call_attention(q, k, v, out, -8.0)
+        check(q, k, v, out, -8.0, peak=1.1)
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("Sq", [1, 40])
 @pytest.mark.parametrize("D", [64, 128, 72])
