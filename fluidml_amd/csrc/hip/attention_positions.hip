@@ -22,7 +22,7 @@ struct AttentionArgs {
   int32_t rows;  // of a key head: queries * group
   float scale2;  // |scale|, in powers of two; its sign is Q's
   float sign, cap, cap2, scale_by_cap, scale_by_cap2;
-  int32_t shaped, q_aligned, out_aligned, by_xcd;
+  int32_t q_aligned, out_aligned, by_xcd;
   FastDiv group_div, kv_div, tiles_div, heads_div;  // query heads of a key head, key heads, tiles of rows, key heads of all sequences
   int2 *ranges;  // documents of every kBlock keys [batch, blocks], or NULL
   int32_t blocks, splits;
@@ -84,15 +84,17 @@ __device__ __forceinline__ Row RowOf(const AttentionArgs &a, const Sequence &s, 
   row.at = s.start + row.i;
   row.document = a.query_documents == nullptr ? 0 : a.query_documents[b * a.query_document_strides[0] + i * a.query_document_strides[1]];
   const bool sees = row.there && row.document >= 0;
+  if (row.document < 0) row.document = -2;
   row.lo = sees ? FirstKey(a, s, row.i) : 0;
-  row.hi = sees ? LastKey(a, s, row.i) : 0;
+  row.hi = sees ? max(LastKey(a, s, row.i), row.lo) : 0;
   row.prefix = sees ? s.prefix : 0;
   row.slope = a.slopes == nullptr ? 0.0f : a.slopes[row.head * a.slope_stride] * kLog2e;
   return row;
 }
 
+// (-1: padding, which no row's document is)
 __device__ __forceinline__ int32_t KeyDocument(const AttentionArgs &a, int b, int32_t j) {
-  return a.key_documents[b * a.key_document_strides[0] + static_cast<int64_t>(j) * a.key_document_strides[1]];
+  return max(a.key_documents[b * a.key_document_strides[0] + static_cast<int64_t>(j) * a.key_document_strides[1]], -1);
 }
 
 __device__ __forceinline__ bool Sees(const AttentionArgs &a, const Row &row, int b, int32_t j) {
@@ -101,19 +103,8 @@ __device__ __forceinline__ bool Sees(const AttentionArgs &a, const Row &row, int
   return sees;
 }
 
-// scale (q . k) capped, in powers of two; PRECISE: to a few roundings of the score itself (a tanh by exponentials is good to a
-// few roundings of the cap, which is far below what 16-bit operands carry)
-template <bool PRECISE>
-__device__ __forceinline__ float Scored(const AttentionArgs &a, float dot) {
-  if (a.cap == 0.0f) return dot * a.scale2;
-  if constexpr (PRECISE) {
-    return a.cap2 * tanhf(dot * a.scale_by_cap);
-  } else {
-    // cap tanh(x) = cap - 2 cap / (1 + exp(2 x))
-    const float e = __builtin_amdgcn_exp2f(dot * a.scale_by_cap2);
-    return a.cap2 - 2.0f * a.cap2 * __builtin_amdgcn_rcpf(1.0f + e);
-  }
-}
+// cap tanh(scale (q . k) / cap), in powers of two
+__device__ __forceinline__ float Capped(const AttentionArgs &a, float dot) { return a.cap2 * tanhf(dot * a.scale_by_cap); }
 
 // One row by one wave, key by key as the definition has it: what a row gets whose sums are not finite.  (A tile's products take in
 // every value of its keys, 0 * infinity among them; here what a query does not see is not read.)
@@ -135,7 +126,7 @@ __device__ __forceinline__ void CarefulRow(const AttentionArgs &a, int b, int kv
     if (sees) {
       s = 0.0f;
       for (int d = 0; d < a.columns; ++d) s += static_cast<float>(q[d * a.q.strides[3]]) * a.sign * static_cast<float>(k[j * a.k.strides[2] + d * a.k.strides[3]]);
-      s = Scored<true>(a, s);
+      s = a.cap == 0.0f ? s * a.scale2 : Capped(a, s);
       if (a.slopes != nullptr) s -= row.slope * fabsf(static_cast<float>(row.at - j));
     }
     const float now = fmaxf(most, WaveReduce(s, MaxOp{}));
@@ -183,6 +174,7 @@ struct Tiles {
   int32_t first, step, end;  // candidates: first, first + step, .. below end
   int32_t base;
   uint64_t mask;
+  int32_t own_document;      // of the lane's candidate: the one document of its keys, or -1
 
   __device__ __forceinline__ void Fill(const AttentionArgs &a, int b) {
     mask = 0;
@@ -192,55 +184,72 @@ struct Tiles {
       if (some && a.ranges != nullptr) {
         const int2 r = a.ranges[static_cast<int64_t>(b) * a.blocks + j / kBlock];
         some = r.y >= least && r.x <= most;
+        own_document = r.x == r.y ? r.x : -1;
       }
       mask = __ballot(some);
       if (mask != 0) return;
       base += kWave * step;
     }
   }
-  // the next tile, or -1
-  __device__ __forceinline__ int32_t Next(const AttentionArgs &a, int b) {
+  // the next tile, or -1; `document`: of all its keys, or -1
+  __device__ __forceinline__ int32_t Next(const AttentionArgs &a, int b, int32_t &document) {
     if (mask == 0) {
       if (base >= end) return -1;
       base += kWave * step;
       Fill(a, b);
       if (mask == 0) return -1;
     }
-    const int32_t tile = base + __builtin_ctzll(mask) * step;
+    const int32_t at = __builtin_ctzll(mask);
     mask &= mask - 1;
-    return tile;
+    document = __builtin_amdgcn_readlane(own_document, at);
+    return base + at * step;
   }
   __device__ __forceinline__ void Start(const AttentionArgs &a, int b) {
+    own_document = -1;
     base = first;
     Fill(a, b);
   }
 };
 
-// Applies scale, cap and bias to the dot products of one row with N keys and hides those it does not see.  `key(e)`: the e-th key.  Returns
-// what the values still are to be multiplied by (scores without cap and bias keep their scale until the exponential, which has
-// a multiplication to spare).
-template <bool PRECISE, int N, typename K>
-__device__ __forceinline__ float Finish(const AttentionArgs &a, const Row &row, int b, bool whole, float (&s)[N], K key) {
+// Applies scale, cap and bias to the dot products of one row with N keys and hides those it does not see.  `key(e)`: the e-th key;
+// `document(e)`: its document.  Returns what the values still are to be multiplied by: scores without bias keep their scale until the
+// exponential, which has a multiplication to spare.  Scores that are the same amount too small are the same to a softmax.
+// PRECISE: the cap to a few roundings of the score itself.  Else cap tanh(x) = cap - 2 cap / (1 + exp(2 x)) without its first
+// term, which is good to a few roundings of the cap: far below what 16-bit operands carry.
+template <bool PRECISE, int N, typename K, typename D>
+__device__ __forceinline__ float Finish(const AttentionArgs &a, const Row &row, bool prefixed, bool whole, bool one_document, float (&s)[N], K key, D document) {
   float by = a.scale2;
-  if (a.shaped) {
-    by = 1.0f;
+  if (a.cap != 0.0f) {
+    if constexpr (PRECISE) {
+      by = 1.0f;
 #pragma unroll
-    for (int e = 0; e < N; ++e) s[e] = Scored<PRECISE>(a, s[e]);
-    if (a.slopes != nullptr) {
+      for (int e = 0; e < N; ++e) s[e] = Capped(a, s[e]);
+    } else {
+      by = 2.0f * a.cap2;
 #pragma unroll
-      for (int e = 0; e < N; ++e) s[e] -= row.slope * fabsf(static_cast<float>(row.at - key(e)));
+      for (int e = 0; e < N; ++e) s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_by_cap2);
+#pragma unroll
+      for (int e = 0; e < N; ++e) s[e] = __builtin_amdgcn_rcpf(-1.0f - s[e]);
     }
   }
+  if (a.slopes != nullptr || by == 0.0f) {  // (no scale: an infinite product is no number, and one that is not seen minus infinity)
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] = s[e] * by - row.slope * fabsf(static_cast<float>(row.at - key(e)));
+    by = 1.0f;
+  }
   if (!whole) {
+    const uint32_t width = static_cast<uint32_t>(row.hi - row.lo);  // (never negative: a window holds a key or the row sees none)
+    if (prefixed) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int32_t j = key(e);
-      s[e] = (j >= row.lo && j < row.hi) || j < row.prefix ? s[e] : -INFINITY;
-    }
-    if (a.key_documents != nullptr) {
+      for (int e = 0; e < N; ++e) s[e] = static_cast<uint32_t>(key(e) - row.lo) < width || key(e) < row.prefix ? s[e] : -INFINITY;
+    } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e) s[e] = KeyDocument(a, b, min(key(e), a.keys - 1)) == row.document ? s[e] : -INFINITY;
+      for (int e = 0; e < N; ++e) s[e] = static_cast<uint32_t>(key(e) - row.lo) < width ? s[e] : -INFINITY;
     }
+  }
+  if (!one_document) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] = document(e) == row.document ? s[e] : -INFINITY;
   }
   return by;
 }
@@ -272,6 +281,19 @@ __device__ __forceinline__ void Settle(Acc (&acc)[N]) {
   asm volatile("s_nop 10");
 #pragma unroll
   for (int n = 0; n < N; ++n) asm volatile("" : "+v"(acc[n]));  // .. and before what reads them
+}
+
+// Asks the compiler for this order of the products that stand before it and of the LDS reads of their operands, READS each: those of the
+// first AHEAD products, then a product and the reads of a later one in turn.  Left alone it reads each operand right before its product.
+template <int AHEAD, int READS, int PRODUCTS>
+__device__ __forceinline__ void ReadAhead() {
+  constexpr int kProduct = 0x8, kRead = 0x100;
+  __builtin_amdgcn_sched_group_barrier(kRead, AHEAD * READS, 0);
+  StaticFor<PRODUCTS - AHEAD>([](auto) __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_group_barrier(kProduct, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, READS, 0);
+  });
+  __builtin_amdgcn_sched_group_barrier(kProduct, AHEAD, 0);
 }
 
 // Eight neighbouring values of a row from column d on, zeros behind the last column.
@@ -322,6 +344,9 @@ __global__ __launch_bounds__(256, WAVES) void AttentionRowsKernel(const Attentio
   constexpr bool kParted = Shape::kParts == 3;
   using E = std::conditional_t<kParted, __bf16, T>;
   constexpr int kParts = Shape::kParts, kSteps = DP / 16, kColumns = DP / 32, kKeyTiles = BK / 32;
+  // operands read ahead of the products: 4096 queries and keys of 32 heads of 128, 330 -> 321 us; at 64 columns the registers cost the third wave
+  // (114 -> 130), at 256 they are not there (472 -> 519)
+  constexpr bool kAhead = !kParted && (DP == 96 || DP == 128);
   __shared__ alignas(16) uint16_t lds[Shape::kValues];
 
   // which rows: a key head's workgroups run on one XCD where that comes out even, its last (with a causal mask: longest) rows first
@@ -395,7 +420,7 @@ __global__ __launch_bounds__(256, WAVES) void AttentionRowsKernel(const Attentio
   if (tiles.most >= 0) {
     tiles.Start(a, b);
   } else {
-    tiles.base = tiles.end, tiles.mask = 0;
+    tiles.base = tiles.end, tiles.mask = 0, tiles.own_document = -1;
   }
 
   // a thread's groups of eight values: key and column group, the same of every tile
@@ -403,7 +428,34 @@ __global__ __launch_bounds__(256, WAVES) void AttentionRowsKernel(const Attentio
   const T *const v_head = static_cast<const T *>(a.v.base) + b * a.v.strides[0] + kv * a.v.strides[1];
   const int last_group = (a.columns - 1) / 8;
   floatx4 staged[kParted ? 2 : 1][kParted ? Shape::kLoads : 1][2];
+  uint32_t offset[kParted ? 1 : 2][kParted ? 1 : Shape::kLoads];  // bytes from a tile's first key, where that fits
+  const bool near = max(a.k.strides[2], a.v.strides[2]) < (1 << 23);
+  if constexpr (!kParted) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+#pragma unroll
+      for (int n = 0; n < Shape::kLoads; ++n) {
+        const int place = (wave * Shape::kLoads + n) * kWave + lane, key = place / (DP / 8);
+        const int group = place % (DP / 8) ^ (m == 0 ? key & Shape::kSwizzleK : 2 * key & Shape::kSwizzleV);
+        offset[m][n] = static_cast<uint32_t>(key) * static_cast<uint32_t>(m == 0 ? a.k.strides[2] : a.v.strides[2]) * 2 + min(group, last_group) * 16;
+      }
+    }
+  }
   auto fetch = [&](int32_t t, int buffer) __attribute__((always_inline)) {
+    if constexpr (!kParted) {
+      if (near && t * BK + BK <= seq.n_keys) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const char *const from = reinterpret_cast<const char *>((m == 0 ? k_head : v_head) + static_cast<int64_t>(t * BK) * (m == 0 ? a.k.strides[2] : a.v.strides[2]));
+#pragma unroll
+          for (int n = 0; n < Shape::kLoads; ++n) {
+            const int32_t to = ((buffer * 2 + m) * Shape::kGroups + (wave * Shape::kLoads + n) * kWave) * 8;
+            LoadToLds(from + offset[m][n], lds + to);
+          }
+        }
+        return;
+      }
+    }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       const T *const from = m == 0 ? k_head : v_head;
@@ -455,11 +507,11 @@ __global__ __launch_bounds__(256, WAVES) void AttentionRowsKernel(const Attentio
   const int v_key = 4 * half + lane % 16 / 4;                                  // V: key ..
   const int v_group = lane / 16 % 2 * 2 + lane % 4 / 2, v_swizzle = 2 * (lane % 16 / 4) & Shape::kSwizzleV;
 
-  int32_t now = tiles.Next(a, b);
+  int32_t now_document = -1, next_document = -1, now = tiles.Next(a, b, now_document);
   int buffer = 0;
   if (now >= 0) fetch(now, 0);
   while (now >= 0) {
-    const int32_t next = tiles.Next(a, b);
+    const int32_t next = tiles.Next(a, b, next_document);
     if constexpr (kParted) {
       __syncthreads();  // everyone is done with the tile before
       store();
@@ -495,17 +547,20 @@ __global__ __launch_bounds__(256, WAVES) void AttentionRowsKernel(const Attentio
           }
         }
       }
+      if constexpr (kAhead) ReadAhead<4, 1, kKeyTiles * kSteps>();
       Settle(dots);
       if constexpr (kParted) Settle(lows);
 #pragma unroll
       for (int e = 0; e < kKeyTiles * 16; ++e) s[e] = kParted ? dots[e / 16][e % 16] + lows[kParted ? e / 16 : 0][e % 16] : dots[e / 16][e % 16];
-      bool whole = (j0 >= all_lo && j0 + BK <= all_hi) || j0 + BK <= seq.prefix;
-      if (a.ranges != nullptr) {
-        const int2 r = a.ranges[static_cast<int64_t>(b) * a.blocks + j0 / kBlock];
-        whole = whole && r.x == r.y && r.x == wave_document;
-      }
-      const int32_t j_lane = j0 + 4 * half;
-      const float by = Finish<kParted>(a, row, b, whole, s, [&](int e) { return j_lane + e / 16 * 32 + e % 16 / 4 * 8 + e % 4; });
+      const bool whole = (j0 >= all_lo && j0 + BK <= all_hi) || j0 + BK <= seq.prefix;
+      const bool one_document = a.ranges == nullptr || (now_document >= 0 && now_document == wave_document);
+      const int32_t j_lane = j0 + 4 * half, ids = one_document ? 0 : KeyDocument(a, b, min(j0 + lane, a.keys - 1));
+      const float by = Finish<kParted>(a, row, seq.prefix > 0, whole, one_document, s, [&](int e) { return j_lane + e / 16 * 32 + e % 16 / 4 * 8 + e % 4; },
+                                       [&](int e) {
+                                         const int from = e / 16 * 32 + e % 16 / 4 * 8 + e % 4;
+                                         const int32_t lower = __builtin_amdgcn_readlane(ids, from), upper = __builtin_amdgcn_readlane(ids, from + 4);
+                                         return half == 0 ? lower : upper;
+                                       });
       float top = s[0];
 #pragma unroll
       for (int e = 1; e < kKeyTiles * 16; ++e) top = fmaxf(top, s[e]);
@@ -570,8 +625,9 @@ __global__ __launch_bounds__(256, WAVES) void AttentionRowsKernel(const Attentio
           for (int e = 0; e < 16; ++e) acc[c][e] += low[e];
         }
       }
+      if constexpr (kAhead) ReadAhead<4, 2, kColumns * kKeyTiles * 2>();
     }
-    now = next;
+    now = next, now_document = next_document;
     if constexpr (!kParted) buffer ^= 1;
   }
 
@@ -686,7 +742,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void AttentionFewKernel(con
     for (int s = 0; s < kSteps; ++s) {
       float x[8] = {};
       const int d = (s * 4 + quarter) * kGroup;
-      if (there) Load8(from, a.q.strides[3], d, min(a.columns, d + kGroup), x);
+      if (a.q_aligned) {  // (no branch around a load: what is not there is read elsewhere in q and made zero)
+        const Group g = *reinterpret_cast<const Group *>((there ? from : static_cast<const T *>(a.q.base)) + min(d, a.columns - kGroup));
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e) x[e] = there && d < a.columns ? static_cast<float>(g[e]) : 0.0f;
+      } else if (there) {
+        Load8(from, a.q.strides[3], d, min(a.columns, d + kGroup), x);
+      }
 #pragma unroll
       for (int e = 0; e < kGroup; ++e) q[s][e] = static_cast<T>(x[e] * a.sign);
     }
@@ -710,7 +772,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void AttentionFewKernel(con
   if (tiles.most >= 0) {
     tiles.Start(a, b);
   } else {
-    tiles.base = tiles.end, tiles.mask = 0;
+    tiles.base = tiles.end, tiles.mask = 0, tiles.own_document = -1;
   }
 
   const T *const k_head = static_cast<const T *>(a.k.base) + b * a.k.strides[0] + kv * a.k.strides[1];
@@ -768,7 +830,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void AttentionFewKernel(con
 #pragma unroll
   for (int c = 0; c < kColumns; ++c) acc[c] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
   float most = -INFINITY, sum = 0.0f;
-  auto work = [&](int32_t tile, int32_t next, auto more) __attribute__((always_inline)) {
+  auto work = [&](int32_t tile, int32_t document, int32_t next, auto more) __attribute__((always_inline)) {
     const int32_t j0 = tile * kKeys;
     float s[kOwn];
     floatx4 dots[kKeyTiles];
@@ -792,13 +854,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void AttentionFewKernel(con
 #pragma unroll
     for (int e = 0; e < kOwn; ++e) s[e] = dots[e / 4][e % 4];
     if constexpr (decltype(more)::value) load_k(next);
-    bool whole = (j0 >= all_lo && j0 + kKeys <= all_hi) || j0 + kKeys <= seq.prefix;
-    if (a.ranges != nullptr) {
-      const int2 r = a.ranges[static_cast<int64_t>(b) * a.blocks + j0 / kBlock];
-      whole = whole && r.x == r.y && r.x == row_document;
-    }
-    const int32_t j_lane = j0 + 4 * quarter;
-    const float by = Finish<kWide>(a, row, b, whole, s, [&](int e) { return j_lane + e / 4 * 16 + e % 4; });
+    const bool whole = (j0 >= all_lo && j0 + kKeys <= all_hi) || j0 + kKeys <= seq.prefix;
+    const bool one_document = a.ranges == nullptr || (document >= 0 && document == row_document);
+    const int32_t j_lane = j0 + 4 * quarter, ids = one_document ? 0 : KeyDocument(a, b, min(j0 + lane % kKeys, a.keys - 1));
+    const float by = Finish<kWide>(a, row, seq.prefix > 0, whole, one_document, s, [&](int e) { return j_lane + e / 4 * 16 + e % 4; },
+                                   [&](int e) { return __shfl(ids, e / 4 * 16 + 4 * quarter + e % 4); });
     float top = s[0];
 #pragma unroll
     for (int e = 1; e < kOwn; ++e) top = fmaxf(top, s[e]);
@@ -840,12 +900,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void AttentionFewKernel(con
     }
     if constexpr (decltype(more)::value) load_v(next);
   };
-  int32_t now = tiles.Next(a, b);
+  int32_t now_document = -1, next_document = -1, now = tiles.Next(a, b, now_document);
   if (now >= 0) {
     load_k(now);
     load_v(now);
-    for (int32_t next; (next = tiles.Next(a, b)) >= 0; now = next) work(now, next, std::true_type{});
-    work(now, -1, std::false_type{});
+    for (int32_t next; (next = tiles.Next(a, b, next_document)) >= 0; now = next, now_document = next_document) work(now, now_document, next, std::true_type{});
+    work(now, now_document, -1, std::false_type{});
   }
 
   asm volatile("s_nop 10");  // (as in Settle: the loop's end is a branch)
@@ -1111,8 +1171,6 @@ int fluidml_hip_attention_positions(const fl_tensor *q, const fl_tensor *k, cons
     a.scale_by_cap = static_cast<float>(scale / scores->cap);
     a.scale_by_cap2 = static_cast<float>(2.0 * log2e * scale / scores->cap);
   }
-  // (no scale: an infinite product is no number, and one that is not seen is still minus infinity)
-  a.shaped = scores->cap > 0.0 || scores->slopes != nullptr || a.scale2 == 0.0f;
   a.q_aligned = Aligned(q) && q->shape[3] % 8 == 0;
   const size_t item = q->dtype == FL_FLOAT32 ? 4 : 2;
   a.out_aligned = IsAligned(out->base, 4 * item) && out->shape[3] % 4 == 0 && out->strides[3] == 1;
