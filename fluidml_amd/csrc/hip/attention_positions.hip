@@ -1086,7 +1086,7 @@ int LaunchRows(const AttentionArgs &a, hipStream_t stream) {
     }
   } else {
     if (a.columns <= 64) {
-      FL_LAUNCH((AttentionRowsKernel<T, 64, 64, 2>), grid, block, 0, stream, a);
+      FL_LAUNCH((AttentionRowsKernel<T, 64, 64, 3>), grid, block, 0, stream, a);
     } else if (a.columns <= 96) {
       FL_LAUNCH((AttentionRowsKernel<T, 96, 64, 2>), grid, block, 0, stream, a);
     } else if (a.columns <= 128) {

@@ -1,5 +1,6 @@
 // The gated feed-forward block: products = act(x . gate + gate_bias) * (x . up + up_bias), out = products . down + down_bias + addend.
 #include <cmath>
+#include <type_traits>
 
 #include "decoder_common.h"
 
@@ -12,40 +13,608 @@ struct GatedArgs {
   void *out;
   int64_t x_strides[2], gate_strides[2], up_strides[2], out_strides[2], addend_strides[2], gate_bias_stride, up_bias_stride;
   int32_t rows, depth, columns, activation;
+  FastDiv row_tiles, column_tiles, group;  // tiles of x, of the weights; tiles of x that are walked together times those of the weights
+  int32_t out_vectors;  // four results of a row in one store
+  int32_t x_direct, weights_direct;  // straight into LDS: 16-byte aligned, and near enough for 32-bit offsets
+  int32_t x_run, gate_run, up_run;   // values of the layout's long side lie side by side
 };
+
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+
+// 1 / (1 + exp(-v)), from exp2 and the reciprocal instruction: a few roundings of itself
+__device__ __forceinline__ float Logistic(float v) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f)); }
 
 __device__ __forceinline__ float Activated(int activation, float v) {
   switch (activation) {
-    case FL_GATE_SILU: return v / (1.0f + expf(-v));
+    case FL_GATE_SILU: return v * Logistic(v);
     case FL_GATE_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-    case FL_GATE_GELU_TANH: return 0.5f * v * (1.0f + tanhf(0.79788456080286536f * (v + 0.044715f * v * v * v)));
+    case FL_GATE_GELU_TANH: return v * Logistic(1.5957691216057308f * (v + 0.044715f * v * v * v));  // 1 + tanh y = 2 / (1 + exp(-2 y))
     case FL_GATE_RELU: return v != v ? v : fmaxf(v, 0.0f);
-    case FL_GATE_SIGMOID: return 1.0f / (1.0f + expf(-v));
+    case FL_GATE_SIGMOID: return Logistic(v);
     default: return v;
   }
 }
 
-// A thread per result.  GATED: two sums and their product; else one sum, a bias and an addend.
+template <typename T>
+__device__ __forceinline__ float BiasAt(const void *bias, int64_t stride, int64_t n) {
+  return bias == nullptr ? 0.0f : static_cast<float>(static_cast<const T *>(bias)[n * stride]);
+}
+
+// The epilogue of one result: biases, the activation and the product, or a bias and an addend.
 template <typename T, bool GATED>
-__global__ __launch_bounds__(256) void GatedSimpleKernel(const GatedArgs a) {
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, m = blockIdx.y;
-  if (n >= a.columns) return;
-  const T *const x = static_cast<const T *>(a.x) + m * a.x_strides[0];
-  const T *const gate = static_cast<const T *>(a.gate) + n * a.gate_strides[1], *const up = static_cast<const T *>(a.up) + n * a.up_strides[1];
-  float g = 0.0f, u = 0.0f;
-  for (int64_t k = 0; k < a.depth; ++k) {
-    const float v = static_cast<float>(x[k * a.x_strides[1]]);
-    g += v * static_cast<float>(gate[k * a.gate_strides[0]]);
-    if constexpr (GATED) u += v * static_cast<float>(up[k * a.up_strides[0]]);
-  }
-  if (a.gate_bias != nullptr) g += static_cast<float>(static_cast<const T *>(a.gate_bias)[n * a.gate_bias_stride]);
+__device__ __forceinline__ void StoreOne(const GatedArgs &a, int32_t m, int32_t n, float g, float u) {
+  g += BiasAt<T>(a.gate_bias, a.gate_bias_stride, n);
   if constexpr (GATED) {
-    if (a.up_bias != nullptr) u += static_cast<float>(static_cast<const T *>(a.up_bias)[n * a.up_bias_stride]);
-    g = Activated(a.activation, g) * u;
+    g = Activated(a.activation, g) * (u + BiasAt<T>(a.up_bias, a.up_bias_stride, n));
   } else if (a.addend != nullptr) {
     g += static_cast<float>(static_cast<const T *>(a.addend)[m * a.addend_strides[0] + n * a.addend_strides[1]]);
   }
   static_cast<T *>(a.out)[m * a.out_strides[0] + n * a.out_strides[1]] = static_cast<T>(g);
+}
+
+// ... of four neighbouring columns of a row
+template <typename T, bool GATED>
+__device__ __forceinline__ void StoreFour(const GatedArgs &a, int32_t m, int32_t n, floatx4 g, floatx4 u) {
+  if (m >= a.rows || n >= a.columns) return;
+  T *const to = static_cast<T *>(a.out) + m * a.out_strides[0] + n * a.out_strides[1];
+  typedef T Vec __attribute__((ext_vector_type(4)));
+  Vec v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int32_t at = min(n + e, a.columns - 1);
+    float x = g[e] + BiasAt<T>(a.gate_bias, a.gate_bias_stride, at);
+    if constexpr (GATED) {
+      x = Activated(a.activation, x) * (u[e] + BiasAt<T>(a.up_bias, a.up_bias_stride, at));
+    } else if (a.addend != nullptr) {
+      x += static_cast<float>(static_cast<const T *>(a.addend)[m * a.addend_strides[0] + at * a.addend_strides[1]]);
+    }
+    v[e] = static_cast<T>(x);
+  }
+  if (a.out_vectors) {
+    *reinterpret_cast<Vec *>(to) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (n + e < a.columns) to[e * a.out_strides[1]] = v[e];
+    }
+  }
+}
+
+// A sum of fp32 products that three bf16 parts cannot carry (an infinity minus itself is no number; parts of the smallest values vanish), again
+// with fp32 products, by the whole wave.
+__device__ __forceinline__ float CarefulDot(const GatedArgs &a, const void *weights, const int64_t (&strides)[2], int32_t m, int32_t n) {
+  const float *const x = static_cast<const float *>(a.x) + m * a.x_strides[0], *const w = static_cast<const float *>(weights) + n * strides[1];
+  float sum = 0.0f;
+  for (int32_t k = threadIdx.x % kWave; k < a.depth; k += kWave) sum += x[k * a.x_strides[1]] * w[k * strides[0]];
+  return GroupSum<64>(sum);
+}
+
+// --------------------------------------------------------------------------------------------------------------------
+// Tiles.  A workgroup owns BM rows of x and BW columns of weights: half of them the gate's and half the up projection's same ones, so that both
+// sums of a result meet in one lane, or (not GATED) BW of one matrix.  Computed transposed, W^T x^T: a lane has one row of the result and
+// four neighbouring columns at a time.  WM x WN x WK waves; WK waves share the depth of a stage and add their sums through LDS.
+// A stage is BK of the depth, in two buffers: the next one is on its way while one is multiplied, one barrier a stage.  Direct: from memory
+// into LDS without a register; otherwise (odd strides and addresses, the last part of a depth that BK does not divide, and fp32,
+// which is split into three bf16 parts on the way) through registers, zeros behind the ends.
+// Weights lie in LDS as they lie in memory, a row for each column of the product (ROWS: a checkpoint's [N, K]) or a row for each of the
+// depth ([K, N], turned by the transposing read).  Groups of 16 bytes are permuted within a row against bank conflicts.
+template <typename T, int BM_, int BW_, int WM_, int WN_, int WK_, int BK_, bool GATED_, bool ROWS_>
+struct TileShape {
+  static constexpr int BM = BM_, BW = BW_, WM = WM_, WN = WN_, WK = WK_, BK = BK_;
+  static constexpr bool GATED = GATED_, ROWS = ROWS_, kParted = std::is_same_v<T, float>;
+  static constexpr int kParts = kParted ? 3 : 1, kWaves = WM * WN * WK, kThreads = kWaves * kWave;
+  static constexpr int BN = GATED ? BW / 2 : BW;           // columns of the result
+  static constexpr int kXGroups = BM * BK / 8, kWGroups = BW * BK / 8;
+  static constexpr int kXLoads = kXGroups / kThreads, kWLoads = kWGroups / kThreads;  // a thread's, in groups of eight values
+  static constexpr int kRowTiles = BM / WM / 32, kWTiles = BW / WN / 32;
+  static constexpr int kXValues = BM * BK, kWValues = BW * BK;
+  static constexpr int kStage = kParts * (kXValues + kWValues);
+  static constexpr int kStages = kParted && kStage * 2 * 2 > 160 * 1024 ? 1 : 2;
+  static constexpr int kLds = kStage * kStages;
+  static_assert(kXGroups % kThreads == 0 && kWGroups % kThreads == 0 && BK % (16 * WK) == 0 && (!GATED || BW / WN == 64), "every thread and wave has the same to do");
+};
+
+// group of eight values in the place of group `group` of row `row`: of x and of ROWS weights (BK values a row), of the others (BW values a row)
+template <int BK>
+__device__ __forceinline__ int SwizzledLong(int row, int group) {
+  return group ^ (row & (BK / 8 - 1) & 7);
+}
+__device__ __forceinline__ int SwizzledWide(int row, int group) { return group ^ (2 * row & 6); }
+
+template <typename E>
+__device__ __forceinline__ floatx16 Mfma32(u32x4 x, u32x4 y, floatx16 acc) {
+  if constexpr (std::is_same_v<E, _Float16>) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(halfx8, x), __builtin_bit_cast(halfx8, y), acc, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), acc, 0, 0, 0);
+  }
+}
+
+// Eight values `stride` apart, the first `n` of which are there; with `run` side by side at any address.
+template <typename T>
+struct Eight {
+  T v[8];
+};
+template <typename T>
+__device__ __forceinline__ Eight<T> LoadEight(const T *from, int64_t stride, int n, bool run) {
+  Eight<T> x;
+  if (run && n >= 8) {
+    __builtin_memcpy(&x, from, sizeof(x));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x.v[e] = e < n ? from[e * stride] : static_cast<T>(0.0f);
+  }
+  return x;
+}
+
+template <typename T, typename Shape>
+__global__ __launch_bounds__(Shape::kThreads, Shape::kThreads == 512 ? 2 : 1) void GatedTileKernel(const GatedArgs a) {
+  using S = Shape;
+  constexpr int BK = S::BK, BW = S::BW, BN = S::BN, kParts = S::kParts;
+  constexpr bool kParted = S::kParted, GATED = S::GATED, ROWS = S::ROWS;
+  using E = std::conditional_t<kParted, __bf16, T>;
+  __shared__ alignas(16) uint16_t lds[S::kLds];
+  const int lane = threadIdx.x % kWave, half = lane / 32, own = lane % 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wk = wave % S::WK, wn = wave / S::WK % S::WN, wm = wave / S::WK / S::WN;
+
+  // workgroups of an XCD (every eighth) work on neighbouring tiles: `group` tiles of rows by all columns, one after the other
+  uint32_t id = blockIdx.x;
+  const uint32_t total = a.row_tiles.divisor * a.column_tiles.divisor, even = total / 8 * 8;
+  if (id < even) id = id % 8 * (total / 8) + id / 8;
+  uint32_t row_tile, column_tile;
+  {
+    const uint32_t g = a.group.Div(id), rest = id - g * a.group.divisor, high = a.group.divisor / a.column_tiles.divisor;
+    const uint32_t here = min(high, a.row_tiles.divisor - g * high);
+    column_tile = rest / here;
+    row_tile = g * high + (rest - column_tile * here);
+  }
+  const int32_t m0 = static_cast<int32_t>(row_tile) * S::BM, n0 = static_cast<int32_t>(column_tile) * BN;
+
+  const T *const x_tile = static_cast<const T *>(a.x) + m0 * a.x_strides[0];
+  const T *const gate_tile = static_cast<const T *>(a.gate) + n0 * a.gate_strides[1];
+  const T *const up_tile = GATED ? static_cast<const T *>(a.up) + n0 * a.up_strides[1] : nullptr;
+
+  // where a thread's groups come from.  x: row and group of the depth.  Weights: column and group of the depth (ROWS), or depth and group of columns
+  uint32_t x_offset[kParted ? 1 : S::kXLoads], w_offset[kParted ? 1 : S::kWLoads];
+  if constexpr (!kParted) {
+#pragma unroll
+    for (int n = 0; n < S::kXLoads; ++n) {
+      const int place = (wave * S::kXLoads + n) * kWave + lane, row = place / (BK / 8), group = SwizzledLong<BK>(row, place % (BK / 8));
+      x_offset[n] = static_cast<uint32_t>(min(row, a.rows - 1 - m0)) * static_cast<uint32_t>(a.x_strides[0]) * 2 + group * 16;
+    }
+#pragma unroll
+    for (int n = 0; n < S::kWLoads; ++n) {
+      const int place = (wave * S::kWLoads + n) * kWave + lane;
+      if constexpr (ROWS) {
+        const int row = place / (BK / 8), group = SwizzledLong<BK>(row, place % (BK / 8));
+        const bool up = GATED && row >= BN;
+        w_offset[n] = static_cast<uint32_t>(min(up ? row - BN : row, a.columns - 1 - n0)) * static_cast<uint32_t>(up ? a.up_strides[1] : a.gate_strides[1]) * 2 + group * 16;
+      } else {
+        const int row = place / (BW / 8), group = SwizzledWide(row, place % (BW / 8));
+        const bool up = GATED && group >= BN / 8;
+        // (columns behind the last: the last group again, whose results are not stored)
+        w_offset[n] = static_cast<uint32_t>(row) * static_cast<uint32_t>(up ? a.up_strides[0] : a.gate_strides[0]) * 2 +
+                      min(up ? group - BN / 8 : group, (a.columns - 1 - n0) / 8) * 16;
+      }
+    }
+  }
+  // (a group is the gate's or the up projection's by its place alone: the same for a whole load of a wave where ROWS, else by lane)
+  Eight<T> x_held[S::kXLoads], w_held[S::kWLoads];
+  auto direct = [&](int32_t k0) __attribute__((always_inline)) { return !kParted && k0 + BK <= a.depth; };
+  auto fetch = [&](int32_t k0, int stage) __attribute__((always_inline)) {
+    uint16_t *const x_to = lds + stage * S::kStage, *const w_to = x_to + kParts * S::kXValues;
+    const bool whole = direct(k0);
+    if (!kParted && whole && a.x_direct) {
+      const char *const from = reinterpret_cast<const char *>(x_tile + k0);
+#pragma unroll
+      for (int n = 0; n < S::kXLoads; ++n) LoadToLds(from + x_offset[kParted ? 0 : n], x_to + (wave * S::kXLoads + n) * kWave * 8);
+    } else {
+#pragma unroll
+      for (int n = 0; n < S::kXLoads; ++n) {
+        const int place = (wave * S::kXLoads + n) * kWave + lane, row = place / (BK / 8), group = SwizzledLong<BK>(row, place % (BK / 8));
+        const int32_t k = k0 + group * 8;
+        x_held[n] = LoadEight<T>(x_tile + min(row, a.rows - 1 - m0) * a.x_strides[0] + k * a.x_strides[1], a.x_strides[1], a.depth - k, a.x_run);
+      }
+    }
+    if (!kParted && whole && a.weights_direct) {
+      const int64_t step = ROWS ? 1 : a.gate_strides[0], up_step = ROWS ? 1 : a.up_strides[0];
+      const char *const gate = reinterpret_cast<const char *>(gate_tile + k0 * step), *const up = reinterpret_cast<const char *>(up_tile + (GATED ? k0 * up_step : 0));
+#pragma unroll
+      for (int n = 0; n < S::kWLoads; ++n) {
+        const int place = (wave * S::kWLoads + n) * kWave + lane;
+        const char *from = gate;
+        if constexpr (GATED && ROWS) {
+          if ((wave * S::kWLoads + n) * kWave / (BK / 8) >= BN) from = up;
+        } else if constexpr (GATED) {
+          if (SwizzledWide(place / (BW / 8), place % (BW / 8)) >= BN / 8) from = up;
+        }
+        LoadToLds(from + w_offset[kParted ? 0 : n], w_to + (wave * S::kWLoads + n) * kWave * 8);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < S::kWLoads; ++n) {
+        const int place = (wave * S::kWLoads + n) * kWave + lane;
+        if constexpr (ROWS) {
+          const int row = place / (BK / 8), group = SwizzledLong<BK>(row, place % (BK / 8));
+          const bool up = GATED && row >= BN;
+          const int64_t along = up ? a.up_strides[0] : a.gate_strides[0], across = up ? a.up_strides[1] : a.gate_strides[1];
+          const int32_t k = k0 + group * 8;
+          w_held[n] = LoadEight<T>((up ? up_tile : gate_tile) + min(up ? row - BN : row, a.columns - 1 - n0) * across + k * along, along, a.depth - k, up ? a.up_run : a.gate_run);
+        } else {
+          const int row = place / (BW / 8), group = SwizzledWide(row, place % (BW / 8));
+          const bool up = GATED && group >= BN / 8;
+          const int64_t along = up ? a.up_strides[0] : a.gate_strides[0], across = up ? a.up_strides[1] : a.gate_strides[1];
+          const int32_t k = k0 + row, c = (up ? group - BN / 8 : group) * 8;
+          w_held[n] = LoadEight<T>((up ? up_tile : gate_tile) + c * across + k * along, across, k < a.depth ? a.columns - n0 - c : 0, up ? a.up_run : a.gate_run);
+        }
+      }
+    }
+  };
+  // what `fetch` left in registers
+  auto store = [&](int32_t k0, int stage) __attribute__((always_inline)) {
+    uint16_t *const x_to = lds + stage * S::kStage, *const w_to = x_to + kParts * S::kXValues;
+    const bool whole = direct(k0);
+    auto put = [&](const Eight<T> &x, uint16_t *to, int values, int place) __attribute__((always_inline)) {
+      if constexpr (kParted) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = x.v[e];
+        u32x4 part[3];
+        SplitParts<3>(f, part);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4 *>(to + p * values + place * 8) = part[p];
+      } else {
+        *reinterpret_cast<u32x4 *>(to + place * 8) = __builtin_bit_cast(u32x4, x);
+      }
+    };
+    if (kParted || !(whole && a.x_direct)) {
+#pragma unroll
+      for (int n = 0; n < S::kXLoads; ++n) put(x_held[n], x_to, S::kXValues, (wave * S::kXLoads + n) * kWave + lane);
+    }
+    if (kParted || !(whole && a.weights_direct)) {
+#pragma unroll
+      for (int n = 0; n < S::kWLoads; ++n) put(w_held[n], w_to, S::kWValues, (wave * S::kWLoads + n) * kWave + lane);
+    }
+  };
+
+  floatx16 acc[S::kRowTiles][S::kWTiles], low[kParted ? S::kRowTiles : 1][kParted ? S::kWTiles : 1];
+#pragma unroll
+  for (int i = 0; i < S::kRowTiles; ++i) {
+#pragma unroll
+    for (int j = 0; j < S::kWTiles; ++j) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f, low[kParted ? i : 0][kParted ? j : 0][e] = 0.0f;
+    }
+  }
+  // column (in LDS) of the wave's j-th tile of weights
+  auto w_column = [&](int j) __attribute__((always_inline)) { return GATED ? j * BN + wn * 32 : wn * S::kWTiles * 32 + j * 32; };
+  auto multiply = [&](int stage) __attribute__((always_inline)) {
+    const uint16_t *const x_from = lds + stage * S::kStage, *const w_from = x_from + kParts * S::kXValues;
+#pragma unroll
+    for (int step = 0; step < BK / 16 / S::WK; ++step) {
+      const int st = step * S::WK + wk;
+      u32x4 x[S::kRowTiles][kParts], w[S::kWTiles][kParts];
+#pragma unroll
+      for (int i = 0; i < S::kRowTiles; ++i) {
+        const int row = (wm * S::kRowTiles + i) * 32 + own;
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) x[i][p] = *reinterpret_cast<const u32x4 *>(x_from + p * S::kXValues + row * BK + SwizzledLong<BK>(row, 2 * st + half) * 8);
+      }
+#pragma unroll
+      for (int j = 0; j < S::kWTiles; ++j) {
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+          if constexpr (ROWS) {
+            const int row = w_column(j) + own;
+            w[j][p] = *reinterpret_cast<const u32x4 *>(w_from + p * S::kWValues + row * BK + SwizzledLong<BK>(row, 2 * st + half) * 8);
+          } else {
+            // sixteen lanes read four of the depth by sixteen columns, and each gets one column's four
+            const int row = st * 16 + half * 8 + lane % 16 / 4, group = w_column(j) / 8 + lane / 16 % 2 * 2 + lane % 4 / 2;
+            uint16_t *const from = const_cast<uint16_t *>(w_from) + p * S::kWValues + row * BW + SwizzledWide(row, group) * 8 + lane % 2 * 4;
+            typedef __attribute__((address_space(3))) shortx4 *Lds;
+            const uint64_t first = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from)));
+            const uint64_t second = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + 4 * BW)));
+            w[j][p] = u32x4{static_cast<uint32_t>(first), static_cast<uint32_t>(first >> 32), static_cast<uint32_t>(second), static_cast<uint32_t>(second >> 32)};
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < S::kWTiles; ++j) {
+#pragma unroll
+        for (int i = 0; i < S::kRowTiles; ++i) {
+          if constexpr (kParted) {
+            MfmaParts<3>(w[j], x[i], acc[i][j], low[i][j]);
+          } else {
+            acc[i][j] = Mfma32<E>(w[j][0], x[i][0], acc[i][j]);
+          }
+        }
+      }
+    }
+  };
+
+  fetch(0, 0);
+  store(0, 0);
+  int stage = 0;
+  for (int32_t k0 = 0; k0 < a.depth; k0 += BK) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // the stage is there for all, and everyone is done with the one before
+    asm volatile("" ::: "memory");
+    const bool more = k0 + BK < a.depth;
+    if constexpr (S::kStages == 2) {
+      if (more) fetch(k0 + BK, stage ^ 1);
+      multiply(stage);
+      if (more) store(k0 + BK, stage ^ 1);
+      stage ^= 1;
+    } else {
+      if (more) fetch(k0 + BK, 0);
+      multiply(0);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (more) store(k0 + BK, 0);
+    }
+  }
+  asm volatile("s_nop 15\ns_nop 3");  // (the last products, across the loop's branch: see Settle in attention_positions.hip)
+#pragma unroll
+  for (int i = 0; i < S::kRowTiles; ++i) {
+#pragma unroll
+    for (int j = 0; j < S::kWTiles; ++j) {
+      asm volatile("" : "+v"(acc[i][j]));
+      if constexpr (kParted) {
+        asm volatile("" : "+v"(low[i][j]));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] += low[i][j][e];
+      }
+    }
+  }
+
+  if constexpr (S::WK > 1) {  // the waves that share the depth: the first adds the others' sums, in their order
+    static_assert(S::WM == 1 && S::WN == 1 && S::kLds >= S::kRowTiles * S::kWTiles * 2 * kWave * 17, "sums fit");
+    float *const sums = reinterpret_cast<float *>(lds);
+    for (int w = 1; w < S::WK; ++w) {
+      __syncthreads();
+      if (wk == w) {
+#pragma unroll
+        for (int i = 0; i < S::kRowTiles; ++i) {
+#pragma unroll
+          for (int j = 0; j < S::kWTiles; ++j) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sums[((i * S::kWTiles + j) * 16 + e) * kWave + lane] = acc[i][j][e];
+          }
+        }
+      }
+      __syncthreads();
+      if (wk == 0) {
+#pragma unroll
+        for (int i = 0; i < S::kRowTiles; ++i) {
+#pragma unroll
+          for (int j = 0; j < S::kWTiles; ++j) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] += sums[((i * S::kWTiles + j) * 16 + e) * kWave + lane];
+          }
+        }
+      }
+    }
+    if (wk != 0) return;
+  }
+
+  constexpr int kResults = GATED ? 1 : S::kWTiles;
+#pragma unroll
+  for (int i = 0; i < S::kRowTiles; ++i) {
+    const int32_t row0 = m0 + (wm * S::kRowTiles + i) * 32;
+#pragma unroll
+    for (int j = 0; j < kResults; ++j) {
+      const int32_t column0 = n0 + (GATED ? wn * 32 : w_column(j));
+      if constexpr (kParted) {
+#pragma unroll
+        for (int w = 0; w < (GATED ? 2 : 1); ++w) {
+          bool bad = false;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) bad = bad || BadSum(acc[i][j + w][e], false);
+          if (!__any(bad)) continue;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int32_t column = column0 + e / 4 * 8 + half * 4 + e % 4;
+            for (uint64_t rest = __ballot(BadSum(acc[i][j + w][e], false) && row0 + own < a.rows && column < a.columns); rest != 0; rest &= rest - 1) {
+              const int who = __builtin_ctzll(rest);
+              const float again = CarefulDot(a, w == 0 ? a.gate : a.up, w == 0 ? a.gate_strides : a.up_strides, row0 + who % 32, column0 + e / 4 * 8 + who / 32 * 4 + e % 4);
+              if (lane == who) acc[i][j + w][e] = again;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const floatx4 g = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+        floatx4 u = {};
+        if constexpr (GATED) u = floatx4{acc[i][1][e], acc[i][1][e + 1], acc[i][1][e + 2], acc[i][1][e + 3]};
+        StoreFour<T, GATED>(a, row0 + own, column0 + e / 4 * 8 + half * 4, g, u);
+      }
+    }
+  }
+}
+
+// --------------------------------------------------------------------------------------------------------------------
+// Few rows (a step of decoding): bound by the bytes of the weights, which go straight into registers, 16 x 16 instructions behind them; the rows
+// of x are the instruction's columns, up to sixteen of them RT times.  A workgroup owns 16 columns of the product (ROWS) or 64, and its eight
+// waves share the depth, each a run of kDepth at a time; their sums meet in LDS, in the order of the waves.  The next run is on
+// its way while one is multiplied.
+// ROWS: a lane loads 16 bytes of the depth of column lane % 16.  Otherwise four columns of each of the depth's values of its quarter of the wave,
+// and turns them around in registers.  fp32 stays fp32: at few rows its products cost less than the bytes.
+template <typename T, bool GATED_, bool ROWS_, int RT_>
+struct FewShape {
+  static constexpr bool GATED = GATED_, ROWS = ROWS_, kWide = std::is_same_v<T, float>;
+  static constexpr int RT = RT_, kMatrices = GATED ? 2 : 1;
+  static constexpr int kGroup = 16 / sizeof(T);                       // values of the depth of a lane in a step
+  static constexpr int kStep = 4 * kGroup;                            // of the depth
+  static constexpr int kSteps = ROWS ? (GATED || RT == 2 ? 4 : 8) : (GATED ? 1 : 2);
+  static constexpr int kDepth = kSteps * kStep;                       // a wave's run
+  static constexpr int kTiles = ROWS ? 1 : 4, kColumns = 16 * kTiles; // tiles of sixteen columns
+  static constexpr int kWaves = 8;
+};
+
+template <typename T, typename Shape>
+__global__ __launch_bounds__(512, 2) void GatedFewKernel(const GatedArgs a) {
+  using S = Shape;
+  constexpr bool GATED = S::GATED, ROWS = S::ROWS, kWide = S::kWide;
+  constexpr int RT = S::RT, kMatrices = S::kMatrices, kGroup = S::kGroup, kSteps = S::kSteps, kTiles = S::kTiles;
+  typedef T Group __attribute__((ext_vector_type(kGroup)));
+  typedef T Four __attribute__((ext_vector_type(4)));
+  typedef T Loose __attribute__((ext_vector_type(kGroup), aligned(sizeof(T))));   // at any address
+  typedef T LooseFour __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  __shared__ float joined[S::kWaves][kMatrices][RT][256];
+  const int lane = threadIdx.x % kWave, own = lane % 16, quarter = lane / 16, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int32_t n0 = static_cast<int32_t>(blockIdx.x) * S::kColumns;
+  const T *const x_own = static_cast<const T *>(a.x);
+  const T *const matrix[2] = {static_cast<const T *>(a.gate), static_cast<const T *>(GATED ? a.up : a.gate)};
+  const int64_t along[2] = {a.gate_strides[0], a.up_strides[0]}, across[2] = {a.gate_strides[1], a.up_strides[1]};
+  const bool runs = a.x_run && a.gate_run && (!GATED || a.up_run) && (ROWS || n0 + S::kColumns <= a.columns);
+
+  struct Run {
+    Group x[kSteps][RT];
+    Group w[ROWS ? kMatrices : 1][ROWS ? kSteps : 1];
+    Four v[ROWS ? 1 : kMatrices][ROWS ? 1 : kSteps][ROWS ? 1 : kGroup];  // [depth][columns]
+  };
+  auto load = [&](Run &r, int32_t k0) __attribute__((always_inline)) {
+    if (runs && k0 + S::kDepth <= a.depth) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int32_t k = k0 + s * S::kStep + quarter * kGroup;
+#pragma unroll
+        for (int m = 0; m < kMatrices; ++m) {
+          if constexpr (ROWS) {
+            r.w[m][s] = *reinterpret_cast<const Loose *>(matrix[m] + min(n0 + own, a.columns - 1) * across[m] + k);
+          } else {
+#pragma unroll
+            for (int e = 0; e < kGroup; ++e) r.v[m][s][e] = *reinterpret_cast<const LooseFour *>(matrix[m] + (k + e) * along[m] + n0 + own * 4);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t) r.x[s][t] = *reinterpret_cast<const Loose *>(x_own + min(t * 16 + own, a.rows - 1) * a.x_strides[0] + k);
+      }
+    } else {  // value by value, zeros behind the ends
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int32_t k = k0 + s * S::kStep + quarter * kGroup;
+#pragma unroll
+        for (int m = 0; m < kMatrices; ++m) {
+          if constexpr (ROWS) {
+            const T *const from = matrix[m] + min(n0 + own, a.columns - 1) * across[m];
+#pragma unroll
+            for (int e = 0; e < kGroup; ++e) r.w[m][s][e] = k + e < a.depth ? from[(k + e) * along[m]] : static_cast<T>(0.0f);
+          } else {
+#pragma unroll
+            for (int e = 0; e < kGroup; ++e) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const int32_t n = n0 + own * 4 + c;
+                r.v[m][s][e][c] = k + e < a.depth && n < a.columns ? matrix[m][(k + e) * along[m] + n * across[m]] : static_cast<T>(0.0f);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          const T *const from = x_own + min(t * 16 + own, a.rows - 1) * a.x_strides[0];
+#pragma unroll
+          for (int e = 0; e < kGroup; ++e) r.x[s][t][e] = k + e < a.depth ? from[(k + e) * a.x_strides[1]] : static_cast<T>(0.0f);
+        }
+      }
+    }
+  };
+  floatx4 acc[kMatrices][kTiles][RT];
+#pragma unroll
+  for (int m = 0; m < kMatrices; ++m) {
+#pragma unroll
+    for (int c = 0; c < kTiles; ++c) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) acc[m][c][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  }
+  auto multiply = [&](const Run &r) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int m = 0; m < kMatrices; ++m) {
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c) {
+          if constexpr (kWide) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float w = ROWS ? r.w[ROWS ? m : 0][ROWS ? s : 0][e] : r.v[ROWS ? 0 : m][ROWS ? 0 : s][ROWS ? 0 : e][c];
+#pragma unroll
+              for (int t = 0; t < RT; ++t) acc[m][c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, r.x[s][t][e], acc[m][c][t], 0, 0, 0);
+            }
+          } else {
+            Group w;
+            if constexpr (ROWS) {
+              w = r.w[m][s];
+            } else {  // column c of eight of the depth
+              typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+              u32x4 turned;
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                const u32x2 first = __builtin_bit_cast(u32x2, r.v[m][s][2 * n]), second = __builtin_bit_cast(u32x2, r.v[m][s][2 * n + 1]);
+                turned[n] = __builtin_amdgcn_perm(second[c / 2], first[c / 2], c % 2 == 0 ? 0x05040100u : 0x07060302u);
+              }
+              w = __builtin_bit_cast(Group, turned);
+            }
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+              if constexpr (std::is_same_v<T, _Float16>) {
+                acc[m][c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, r.x[s][t], acc[m][c][t], 0, 0, 0);
+              } else {
+                acc[m][c][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, r.x[s][t], acc[m][c][t], 0, 0, 0);
+              }
+            }
+          }
+        }
+      }
+    }
+  };
+
+  constexpr int32_t kAll = S::kWaves * S::kDepth;
+  Run r;
+  int32_t k0 = wave * S::kDepth;
+  if (k0 < a.depth) {
+    load(r, k0);
+    for (; k0 + kAll < a.depth; k0 += kAll) {
+      Run next;
+      load(next, k0 + kAll);
+      multiply(r);
+      r = next;
+    }
+    multiply(r);
+  }
+  asm volatile("s_nop 10");  // (the last products, across the loop's branch: see Settle in attention_positions.hip)
+#pragma unroll
+  for (int c = 0; c < kTiles; ++c) {
+    if (c > 0) __syncthreads();
+#pragma unroll
+    for (int m = 0; m < kMatrices; ++m) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        asm volatile("" : "+v"(acc[m][c][t]));
+        *reinterpret_cast<floatx4 *>(&joined[wave][m][t][lane * 4]) = acc[m][c][t];
+      }
+    }
+    __syncthreads();
+    for (int at = threadIdx.x; at < RT * 256; at += 512) {
+      // row `row` of x by column `place` of the tile: register place % 4 of lane (place / 4) * 16 + row
+      const int t = at / 256, row = at % 256 / 16, place = at % 16, from = ((place / 4) * 16 + row) * 4 + place % 4;
+      const int32_t m = t * 16 + row, n = n0 + (ROWS ? place : place * 4 + c);
+      if (m >= a.rows || n >= a.columns) continue;
+      float g = 0.0f, u = 0.0f;
+#pragma unroll
+      for (int w = 0; w < S::kWaves; ++w) {
+        g += joined[w][0][t][from];
+        if constexpr (GATED) u += joined[w][kMatrices - 1][t][from];
+      }
+      StoreOne<T, GATED>(a, m, n, g, u);
+    }
+  }
 }
 
 int CheckMatrix(const fl_tensor *t, int32_t dtype, int64_t rows, int64_t columns, bool result = false) {
@@ -75,6 +644,43 @@ void Set(const fl_tensor *t, int64_t (&strides)[2]) {
   for (int i = 0; i < 2; ++i) strides[i] = t == nullptr ? 0 : t->strides[i];
 }
 
+bool Aligned(const fl_tensor *t, int unit) {
+  const int64_t group = static_cast<int64_t>(16 / (t->dtype == FL_FLOAT32 ? 4 : 2));
+  return IsAligned(t->base, 16) && t->strides[unit] == 1 && t->strides[1 - unit] % group == 0 && t->strides[1 - unit] < (1 << 22);
+}
+
+template <typename T, typename Shape>
+int LaunchTiles(GatedArgs &a, hipStream_t stream) {
+  const int64_t rows = (a.rows + Shape::BM - 1) / Shape::BM, columns = (a.columns + Shape::BN - 1) / Shape::BN;
+  if (rows * columns > INT32_MAX / 16) return FL_ERR_TOO_LARGE;
+  a.row_tiles = FastDiv(static_cast<uint32_t>(rows));
+  a.column_tiles = FastDiv(static_cast<uint32_t>(columns));
+  a.group = FastDiv(static_cast<uint32_t>(std::min<int64_t>(rows, 8) * columns));
+  FL_LAUNCH((GatedTileKernel<T, Shape>), dim3(static_cast<uint32_t>(rows * columns)), dim3(Shape::kThreads), 0, stream, a);
+  return LaunchStatus();
+}
+
+template <typename T, typename Shape>
+int LaunchFew(const GatedArgs &a, hipStream_t stream) {
+  FL_LAUNCH((GatedFewKernel<T, Shape>), dim3((a.columns + Shape::kColumns - 1) / Shape::kColumns), dim3(512), 0, stream, a);
+  return LaunchStatus();
+}
+
+template <typename T, bool GATED, bool ROWS>
+int LaunchLayout(GatedArgs &a, hipStream_t stream) {
+  if (a.rows <= 16) return LaunchFew<T, FewShape<T, GATED, ROWS, 1>>(a, stream);
+  if (a.rows <= 32) return LaunchFew<T, FewShape<T, GATED, ROWS, 2>>(a, stream);
+  auto tiles = [&](int64_t bm, int64_t bw) { return (a.rows + bm - 1) / bm * ((a.columns + bw / (GATED ? 2 : 1) - 1) / (bw / (GATED ? 2 : 1))); };
+  if constexpr (std::is_same_v<T, float>) {
+    if (tiles(128, 128) >= 256) return LaunchTiles<T, TileShape<T, 128, 128, 2, 2, 1, 32, GATED, ROWS>>(a, stream);
+    return LaunchTiles<T, TileShape<T, 32, 64, 1, 1, 4, 64, GATED, ROWS>>(a, stream);
+  } else {
+    if (tiles(256, 256) >= 200) return LaunchTiles<T, TileShape<T, 256, 256, 2, 4, 1, 64, GATED, ROWS>>(a, stream);
+    if (tiles(128, 128) >= 256) return LaunchTiles<T, TileShape<T, 128, 128, 2, 2, 1, 64, GATED, ROWS>>(a, stream);
+    return LaunchTiles<T, TileShape<T, 64, 64, 1, 1, 4, 64, GATED, ROWS>>(a, stream);
+  }
+}
+
 // out = act(x . gate + gate_bias) * (x . up + up_bias), or with `up` NULL: x . gate + gate_bias + addend
 int Contract(const fl_tensor *x, const fl_tensor *gate, const fl_tensor *up, const fl_tensor *gate_bias, const fl_tensor *up_bias, const fl_tensor *addend,
              const fl_tensor *out, int32_t activation, hipStream_t stream) {
@@ -89,18 +695,21 @@ int Contract(const fl_tensor *x, const fl_tensor *gate, const fl_tensor *up, con
   a.up_bias_stride = up_bias == nullptr ? 0 : up_bias->strides[0];
   a.rows = static_cast<int32_t>(x->shape[0]), a.depth = static_cast<int32_t>(x->shape[1]), a.columns = static_cast<int32_t>(gate->shape[1]);
   a.activation = activation;
-  if (a.rows > 65535) return FL_ERR_TOO_LARGE;
-  const dim3 grid((a.columns + 255) / 256, a.rows);
-  FL_CHECK(ForDecoderType(x->dtype, [&](auto type) {
+  // the layout that the weights share, or that of a checkpoint; a matrix that has another is read value by value
+  const bool wide = gate->strides[1] == 1 && (up == nullptr || up->strides[1] == 1) && !(gate->strides[0] == 1 && gate->shape[1] > 1 && gate->shape[0] == 1);
+  const int unit = wide ? 1 : 0;
+  a.x_direct = Aligned(x, 1);
+  a.weights_direct = Aligned(gate, unit) && (up == nullptr || Aligned(up, unit)) && (!wide || a.columns % 8 == 0);
+  a.x_run = x->strides[1] == 1;
+  a.gate_run = gate->strides[unit] == 1;
+  a.up_run = up != nullptr && up->strides[unit] == 1;
+  const size_t item = x->dtype == FL_FLOAT32 ? 4 : 2;
+  a.out_vectors = out->strides[1] == 1 && out->strides[0] % 4 == 0 && a.columns % 4 == 0 && IsAligned(out->base, 4 * item);
+  return ForDecoderType(x->dtype, [&](auto type) {
     using T = decltype(type);
-    if (up != nullptr) {
-      FL_LAUNCH((GatedSimpleKernel<T, true>), grid, dim3(256), 0, stream, a);
-    } else {
-      FL_LAUNCH((GatedSimpleKernel<T, false>), grid, dim3(256), 0, stream, a);
-    }
-    return FL_OK;
-  }));
-  return LaunchStatus();
+    if (up != nullptr) return wide ? LaunchLayout<T, true, false>(a, stream) : LaunchLayout<T, true, true>(a, stream);
+    return wide ? LaunchLayout<T, false, false>(a, stream) : LaunchLayout<T, false, true>(a, stream);
+  });
 }
 
 }  // namespace

@@ -70,6 +70,80 @@ def test_gated_matmul(device, dtype, turned, M, K, N):
     check(out, want, oracle.rounded(bound, want, kind))
 
 
+def kernels(run):
+    """Names of what run(stream) launches."""
+    from tests.util import launches
+
+    run(None)
+    return [name for name, _ in launches(run)]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("turned", [True, False], ids=["rows", "columns"])
+@pytest.mark.parametrize("M,K,N,tile", [
+    (2003, 200, 1100, 128), (2100, 71, 1111, 128),    # tiles of 128 rows: columns, depth and rows that they do not divide
+    (3400, 136, 2000, 256), (3333, 70, 1999, 256), (3500, 64, 1984, 256),
+])
+def test_gated_matmul_many_rows(device, dtype, turned, M, K, N, tile):
+    import torch
+
+    print("[case]", dtype, turned, M, K, N, flush=True)
+    kind = dtype_of(dtype)
+    x, gate, up, gb, ub = make(device, kind, M, K, N, turned, M % 2 == 1)
+    out = torch.full((M, N), 7.0, device=device, dtype=kind)
+    name, = kernels(lambda stream: call(x, gate, up, gb, ub, out, "silu", stream))
+    if dtype != "fp32" or tile == 128:
+        assert f"Li{tile}ELi{tile}E" in name
+    out.fill_(7.0)
+    call(x, gate, up, gb, ub, out, "silu")
+    want, bound = oracle.gated(x, gate, up, gb, ub, "silu")
+    check(out, want, oracle.rounded(bound, want, kind))
+    # one matrix, from the products on
+    down = (torch.randn(K, N, device=device) * N ** -0.5).to(kind).t()
+    if not turned:
+        down = down.contiguous()
+    addend, products, back = torch.randn(M, K, device=device).to(kind), torch.empty_like(out), torch.full((M, K), 7.0, device=device, dtype=kind)
+    call_block(x, gate, up, gb, ub, down, None, addend, products, back, "silu")
+    assert torch.equal(products, out)
+    h, d = products.double().cpu(), down.double().cpu()
+    want = h @ d + addend.double().cpu()
+    check(back, want, oracle.rounded(2.0 ** -24 * (N + 4) * (h.abs() @ d.abs()) + 2.0 ** -24 * 2 * (want.abs() + addend.double().cpu().abs()), want, kind))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_gated_down_many_rows(device, dtype):
+    """The projection back in the largest tiles, with a bias."""
+    import torch
+
+    kind = dtype_of(dtype)
+    M, K, N, Oc = 3400, 64, 72, 4000
+    x, gate, up, gb, ub = make(device, kind, M, K, N, True, True)
+    for turned in (True, False):
+        down = (torch.randn(Oc, N, device=device) * N ** -0.5).to(kind).t()
+        if not turned:
+            down = down.contiguous()
+        bias, products, out = torch.randn(Oc, device=device).to(kind), torch.empty(M, N, device=device, dtype=kind), torch.empty(M, Oc, device=device, dtype=kind)
+        names = kernels(lambda stream: call_block(x, gate, up, gb, ub, down, bias, None, products, out, "gelu", stream))
+        assert dtype == "fp32" or "Li256ELi256E" in names[1]
+        h, d = products.double().cpu(), down.double().cpu()
+        want = h @ d + bias.double().cpu()
+        check(out, want, oracle.rounded(2.0 ** -24 * (N + 4) * (h.abs() @ d.abs()) + 2.0 ** -24 * 2 * (want.abs() + bias.double().cpu().abs()), want, kind))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_gated_many_rows_not_finite(device, dtype):
+    import torch
+
+    x, gate, up, _, _ = make(device, dtype_of(dtype), 3400, 72, 2000, True, False)
+    gate[50, 7], up[3, 1960], x[3399, 71], x[5, 0] = float("nan"), float("inf"), float("nan"), -float("inf")
+    out = torch.empty(3400, 2000, device=device, dtype=x.dtype)
+    call(x, gate, up, None, None, out, "relu")
+    want, bound = oracle.gated(x, gate, up, None, None, "relu")
+    assert torch.equal(out.isnan().cpu(), want.isnan()) and torch.equal(out.isinf().cpu(), want.isinf())
+    fine = want.isfinite()
+    assert ((out.double().cpu() - want).abs() <= oracle.rounded(torch.nan_to_num(bound, nan=0.0, posinf=0.0) + 1e-6 * 72, want, x.dtype))[fine].all()
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("kind", oracle.ACTIVATIONS)
 def test_gated_activations(device, dtype, kind):
