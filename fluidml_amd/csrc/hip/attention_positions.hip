@@ -272,17 +272,6 @@ __device__ __forceinline__ u32x4 Pack8(const float *x) {
   return __builtin_bit_cast(u32x4, v);
 }
 
-// Waits until matrix instructions have written these.  The compiler does this where it sees the result read in the same basic block; across a
-// branch (scores that are capped or not, tiles that are masked or not) it has left it out, and the last scores were read too early.
-template <int N, typename Acc>
-__device__ __forceinline__ void Settle(Acc (&acc)[N]) {
-#pragma unroll
-  for (int n = 0; n < N; ++n) asm volatile("" : "+v"(acc[n]));  // behind the products ..
-  asm volatile("s_nop 10");
-#pragma unroll
-  for (int n = 0; n < N; ++n) asm volatile("" : "+v"(acc[n]));  // .. and before what reads them
-}
-
 // Asks the compiler for this order of the products that stand before it and of the LDS reads of their operands, READS each: those of the
 // first AHEAD products, then a product and the reads of a later one in turn.  Left alone it reads each operand right before its product.
 template <int AHEAD, int READS, int PRODUCTS>
@@ -631,7 +620,7 @@ __global__ __launch_bounds__(256, WAVES) void AttentionRowsKernel(const Attentio
     if constexpr (!kParted) buffer ^= 1;
   }
 
-  asm volatile("s_nop 10");  // (as in Settle: the loop's end is a branch)
+  SettleAcrossBranch();
   Settle(acc);
   sum = AcrossHalves(sum, SumOp{});
   const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -908,7 +897,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void AttentionFewKernel(con
     work(now, now_document, -1, std::false_type{});
   }
 
-  asm volatile("s_nop 10");  // (as in Settle: the loop's end is a branch)
+  SettleAcrossBranch();
   Settle(acc);
   // the waves' sums, each as far behind the common maximum as its own
   sum = AcrossRows(AcrossHalves(sum, SumOp{}), SumOp{});

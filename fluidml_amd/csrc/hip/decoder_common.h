@@ -61,6 +61,23 @@ __device__ __forceinline__ void LoadToLds(const void *from, void *to) {
   __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void *)to, 16, 0, 0);
 #endif
 }
+
+// Waits until matrix instructions (of up to 16 passes) have written their results.  The compiler does this where it sees them read in the same basic
+// block; across a branch (scores that are capped or not, the end of a loop) it has left it out, and the last results were read
+// before they were there.  For the block behind such a branch:
+__device__ __forceinline__ void SettleAcrossBranch() {
+  asm volatile("s_nop 10");
+  __builtin_amdgcn_sched_barrier(0);
+}
+// ... and for results of this block that are read behind the next branch
+template <int N, typename Acc>
+__device__ __forceinline__ void Settle(Acc (&acc)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) asm volatile("" : "+v"(acc[n]));  // behind the products ..
+  asm volatile("s_nop 10");
+#pragma unroll
+  for (int n = 0; n < N; ++n) asm volatile("" : "+v"(acc[n]));  // .. and before what reads them
+}
 #endif
 
 }  // namespace fl

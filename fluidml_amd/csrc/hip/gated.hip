@@ -111,8 +111,9 @@ struct TileShape {
   static constexpr int kRowTiles = BM / WM / 32, kWTiles = BW / WN / 32;
   static constexpr int kXValues = BM * BK, kWValues = BW * BK;
   static constexpr int kStage = kParts * (kXValues + kWValues);
-  static constexpr int kStages = kParted && kStage * 2 * 2 > 160 * 1024 ? 1 : 2;
-  static constexpr int kLds = kStage * kStages;
+  static constexpr int kLds = kStage * 2;
+  static constexpr bool kLarge = BM == 256;             // direct loads only
+  static constexpr int kAhead = WK > 1 ? 4 : 1;         // stages on their way in registers
   static_assert(kXGroups % kThreads == 0 && kWGroups % kThreads == 0 && BK % (16 * WK) == 0 && (!GATED || BW / WN == 64), "every thread and wave has the same to do");
 };
 
@@ -132,20 +133,16 @@ __device__ __forceinline__ floatx16 Mfma32(u32x4 x, u32x4 y, floatx16 acc) {
   }
 }
 
-// Eight values `stride` apart, the first `n` of which are there; with `run` side by side at any address.
+// Eight values `stride` apart, the first `n` of which are there.
 template <typename T>
 struct Eight {
   T v[8];
 };
 template <typename T>
-__device__ __forceinline__ Eight<T> LoadEight(const T *from, int64_t stride, int n, bool run) {
+__device__ __forceinline__ Eight<T> LoadEight(const T *from, int64_t stride, int n) {
   Eight<T> x;
-  if (run && n >= 8) {
-    __builtin_memcpy(&x, from, sizeof(x));
-  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x.v[e] = e < n ? from[e * stride] : static_cast<T>(0.0f);
-  }
+  for (int e = 0; e < 8; ++e) x.v[e] = e < n ? from[e * stride] : static_cast<T>(0.0f);
   return x;
 }
 
@@ -201,81 +198,111 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::kThreads == 512 ? 2 : 1) vo
     }
   }
   // (a group is the gate's or the up projection's by its place alone: the same for a whole load of a wave where ROWS, else by lane)
-  Eight<T> x_held[S::kXLoads], w_held[S::kWLoads];
-  auto direct = [&](int32_t k0) __attribute__((always_inline)) { return !kParted && k0 + BK <= a.depth; };
-  auto fetch = [&](int32_t k0, int stage) __attribute__((always_inline)) {
-    uint16_t *const x_to = lds + stage * S::kStage, *const w_to = x_to + kParts * S::kXValues;
-    const bool whole = direct(k0);
-    if (!kParted && whole && a.x_direct) {
-      const char *const from = reinterpret_cast<const char *>(x_tile + k0);
+  auto direct = [&](int32_t k0) __attribute__((always_inline)) { return S::kLarge || (!kParted && S::kAhead == 1 && k0 + BK <= a.depth); };
+  auto fetch_direct = [&](int32_t k0, int stage, bool x, bool weights) __attribute__((always_inline)) {
+    if constexpr (!kParted) {
+      uint16_t *const x_to = lds + stage * S::kStage, *const w_to = x_to + kParts * S::kXValues;
+      if (x) {
+        const char *const from = reinterpret_cast<const char *>(x_tile + k0);
 #pragma unroll
-      for (int n = 0; n < S::kXLoads; ++n) LoadToLds(from + x_offset[kParted ? 0 : n], x_to + (wave * S::kXLoads + n) * kWave * 8);
-    } else {
-#pragma unroll
-      for (int n = 0; n < S::kXLoads; ++n) {
-        const int place = (wave * S::kXLoads + n) * kWave + lane, row = place / (BK / 8), group = SwizzledLong<BK>(row, place % (BK / 8));
-        const int32_t k = k0 + group * 8;
-        x_held[n] = LoadEight<T>(x_tile + min(row, a.rows - 1 - m0) * a.x_strides[0] + k * a.x_strides[1], a.x_strides[1], a.depth - k, a.x_run);
+        for (int n = 0; n < S::kXLoads; ++n) LoadToLds(from + x_offset[n], x_to + (wave * S::kXLoads + n) * kWave * 8);
       }
-    }
-    if (!kParted && whole && a.weights_direct) {
-      const int64_t step = ROWS ? 1 : a.gate_strides[0], up_step = ROWS ? 1 : a.up_strides[0];
-      const char *const gate = reinterpret_cast<const char *>(gate_tile + k0 * step), *const up = reinterpret_cast<const char *>(up_tile + (GATED ? k0 * up_step : 0));
+      if (weights) {
+        const int64_t step = ROWS ? 1 : a.gate_strides[0], up_step = ROWS ? 1 : a.up_strides[0];
+        const char *const gate = reinterpret_cast<const char *>(gate_tile + k0 * step), *const up = reinterpret_cast<const char *>(up_tile + (GATED ? k0 * up_step : 0));
 #pragma unroll
-      for (int n = 0; n < S::kWLoads; ++n) {
-        const int place = (wave * S::kWLoads + n) * kWave + lane;
-        const char *from = gate;
-        if constexpr (GATED && ROWS) {
-          if ((wave * S::kWLoads + n) * kWave / (BK / 8) >= BN) from = up;
-        } else if constexpr (GATED) {
-          if (SwizzledWide(place / (BW / 8), place % (BW / 8)) >= BN / 8) from = up;
-        }
-        LoadToLds(from + w_offset[kParted ? 0 : n], w_to + (wave * S::kWLoads + n) * kWave * 8);
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < S::kWLoads; ++n) {
-        const int place = (wave * S::kWLoads + n) * kWave + lane;
-        if constexpr (ROWS) {
-          const int row = place / (BK / 8), group = SwizzledLong<BK>(row, place % (BK / 8));
-          const bool up = GATED && row >= BN;
-          const int64_t along = up ? a.up_strides[0] : a.gate_strides[0], across = up ? a.up_strides[1] : a.gate_strides[1];
-          const int32_t k = k0 + group * 8;
-          w_held[n] = LoadEight<T>((up ? up_tile : gate_tile) + min(up ? row - BN : row, a.columns - 1 - n0) * across + k * along, along, a.depth - k, up ? a.up_run : a.gate_run);
-        } else {
-          const int row = place / (BW / 8), group = SwizzledWide(row, place % (BW / 8));
-          const bool up = GATED && group >= BN / 8;
-          const int64_t along = up ? a.up_strides[0] : a.gate_strides[0], across = up ? a.up_strides[1] : a.gate_strides[1];
-          const int32_t k = k0 + row, c = (up ? group - BN / 8 : group) * 8;
-          w_held[n] = LoadEight<T>((up ? up_tile : gate_tile) + c * across + k * along, across, k < a.depth ? a.columns - n0 - c : 0, up ? a.up_run : a.gate_run);
+        for (int n = 0; n < S::kWLoads; ++n) {
+          const int place = (wave * S::kWLoads + n) * kWave + lane;
+          const char *from = gate;
+          if constexpr (GATED && ROWS) {
+            if ((wave * S::kWLoads + n) * kWave / (BK / 8) >= BN) from = up;
+          } else if constexpr (GATED) {
+            if (SwizzledWide(place / (BW / 8), place % (BW / 8)) >= BN / 8) from = up;
+          }
+          LoadToLds(from + w_offset[n], w_to + (wave * S::kWLoads + n) * kWave * 8);
         }
       }
     }
   };
-  // what `fetch` left in registers
-  auto store = [&](int32_t k0, int stage) __attribute__((always_inline)) {
+  // through registers: whole runs of eight where they lie side by side, without a branch around a load; else value by value, zeros behind the ends
+  struct Held {
+    Eight<T> x[S::kXLoads], w[S::kWLoads];
+  };
+  auto fetch = [&](Held &held, int32_t k0, bool x, bool weights) __attribute__((always_inline)) {
+    const bool whole = k0 + BK <= a.depth;
+    if (x) {
+      auto at = [&](int n, int32_t &k) __attribute__((always_inline)) {
+        const int place = (wave * S::kXLoads + n) * kWave + lane, row = place / (BK / 8), group = SwizzledLong<BK>(row, place % (BK / 8));
+        k = k0 + group * 8;
+        return x_tile + min(row, a.rows - 1 - m0) * a.x_strides[0] + k * a.x_strides[1];
+      };
+      int32_t k;
+      if (whole && a.x_run) {
+#pragma unroll
+        for (int n = 0; n < S::kXLoads; ++n) __builtin_memcpy(&held.x[n], at(n, k), sizeof(Eight<T>));
+      } else {
+#pragma unroll
+        for (int n = 0; n < S::kXLoads; ++n) {
+          const T *const from = at(n, k);
+          held.x[n] = LoadEight<T>(from, a.x_strides[1], a.depth - k);
+        }
+      }
+    }
+    if (weights) {
+      // `there`: values of the group that are
+      auto at = [&](int n, int64_t &stride, int32_t &there) __attribute__((always_inline)) {
+        const int place = (wave * S::kWLoads + n) * kWave + lane;
+        const int row = ROWS ? place / (BK / 8) : place / (BW / 8);
+        const int group = ROWS ? SwizzledLong<BK>(row, place % (BK / 8)) : SwizzledWide(row, place % (BW / 8));
+        const bool up = GATED && (ROWS ? row >= BN : group >= BN / 8);
+        const int64_t along = up ? a.up_strides[0] : a.gate_strides[0], across = up ? a.up_strides[1] : a.gate_strides[1];
+        const T *const from = up ? up_tile : gate_tile;
+        if constexpr (ROWS) {
+          const int32_t k = k0 + group * 8;
+          stride = along, there = a.depth - k;
+          return from + min(up ? row - BN : row, a.columns - 1 - n0) * across + k * along;
+        } else {
+          const int32_t k = k0 + row, c = (up ? group - BN / 8 : group) * 8;
+          stride = across, there = k < a.depth ? a.columns - n0 - c : 0;
+          return from + c * across + k * along;
+        }
+      };
+      int64_t stride;
+      int32_t there;
+      if (whole && a.gate_run && (!GATED || a.up_run) && (ROWS || n0 + BN <= a.columns)) {
+#pragma unroll
+        for (int n = 0; n < S::kWLoads; ++n) __builtin_memcpy(&held.w[n], at(n, stride, there), sizeof(Eight<T>));
+      } else {
+#pragma unroll
+        for (int n = 0; n < S::kWLoads; ++n) {
+          const T *const from = at(n, stride, there);
+          held.w[n] = LoadEight<T>(from, stride, there);
+        }
+      }
+    }
+  };
+  auto store = [&](const Held &held, int stage, bool x, bool weights) __attribute__((always_inline)) {
     uint16_t *const x_to = lds + stage * S::kStage, *const w_to = x_to + kParts * S::kXValues;
-    const bool whole = direct(k0);
-    auto put = [&](const Eight<T> &x, uint16_t *to, int values, int place) __attribute__((always_inline)) {
+    auto put = [&](const Eight<T> &v, uint16_t *to, int values, int place) __attribute__((always_inline)) {
       if constexpr (kParted) {
         float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = x.v[e];
+        for (int e = 0; e < 8; ++e) f[e] = v.v[e];
         u32x4 part[3];
         SplitParts<3>(f, part);
 #pragma unroll
         for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4 *>(to + p * values + place * 8) = part[p];
       } else {
-        *reinterpret_cast<u32x4 *>(to + place * 8) = __builtin_bit_cast(u32x4, x);
+        *reinterpret_cast<u32x4 *>(to + place * 8) = __builtin_bit_cast(u32x4, v);
       }
     };
-    if (kParted || !(whole && a.x_direct)) {
+    if (x) {
 #pragma unroll
-      for (int n = 0; n < S::kXLoads; ++n) put(x_held[n], x_to, S::kXValues, (wave * S::kXLoads + n) * kWave + lane);
+      for (int n = 0; n < S::kXLoads; ++n) put(held.x[n], x_to, S::kXValues, (wave * S::kXLoads + n) * kWave + lane);
     }
-    if (kParted || !(whole && a.weights_direct)) {
+    if (weights) {
 #pragma unroll
-      for (int n = 0; n < S::kWLoads; ++n) put(w_held[n], w_to, S::kWValues, (wave * S::kWLoads + n) * kWave + lane);
+      for (int n = 0; n < S::kWLoads; ++n) put(held.w[n], w_to, S::kWValues, (wave * S::kWLoads + n) * kWave + lane);
     }
   };
 
@@ -290,73 +317,119 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::kThreads == 512 ? 2 : 1) vo
   }
   // column (in LDS) of the wave's j-th tile of weights
   auto w_column = [&](int j) __attribute__((always_inline)) { return GATED ? j * BN + wn * 32 : wn * S::kWTiles * 32 + j * 32; };
-  auto multiply = [&](int stage) __attribute__((always_inline)) {
+  struct Operands {
+    u32x4 x[S::kRowTiles][kParts], w[S::kWTiles][kParts];
+  };
+  auto read = [&](Operands &o, int stage, int step) __attribute__((always_inline)) {
     const uint16_t *const x_from = lds + stage * S::kStage, *const w_from = x_from + kParts * S::kXValues;
+    const int st = step * S::WK + wk;
 #pragma unroll
-    for (int step = 0; step < BK / 16 / S::WK; ++step) {
-      const int st = step * S::WK + wk;
-      u32x4 x[S::kRowTiles][kParts], w[S::kWTiles][kParts];
+    for (int j = 0; j < S::kWTiles; ++j) {
 #pragma unroll
-      for (int i = 0; i < S::kRowTiles; ++i) {
-        const int row = (wm * S::kRowTiles + i) * 32 + own;
-#pragma unroll
-        for (int p = 0; p < kParts; ++p) x[i][p] = *reinterpret_cast<const u32x4 *>(x_from + p * S::kXValues + row * BK + SwizzledLong<BK>(row, 2 * st + half) * 8);
-      }
-#pragma unroll
-      for (int j = 0; j < S::kWTiles; ++j) {
-#pragma unroll
-        for (int p = 0; p < kParts; ++p) {
-          if constexpr (ROWS) {
-            const int row = w_column(j) + own;
-            w[j][p] = *reinterpret_cast<const u32x4 *>(w_from + p * S::kWValues + row * BK + SwizzledLong<BK>(row, 2 * st + half) * 8);
-          } else {
-            // sixteen lanes read four of the depth by sixteen columns, and each gets one column's four
-            const int row = st * 16 + half * 8 + lane % 16 / 4, group = w_column(j) / 8 + lane / 16 % 2 * 2 + lane % 4 / 2;
-            uint16_t *const from = const_cast<uint16_t *>(w_from) + p * S::kWValues + row * BW + SwizzledWide(row, group) * 8 + lane % 2 * 4;
-            typedef __attribute__((address_space(3))) shortx4 *Lds;
-            const uint64_t first = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from)));
-            const uint64_t second = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + 4 * BW)));
-            w[j][p] = u32x4{static_cast<uint32_t>(first), static_cast<uint32_t>(first >> 32), static_cast<uint32_t>(second), static_cast<uint32_t>(second >> 32)};
-          }
+      for (int p = 0; p < kParts; ++p) {
+        if constexpr (ROWS) {
+          const int row = w_column(j) + own;
+          o.w[j][p] = *reinterpret_cast<const u32x4 *>(w_from + p * S::kWValues + row * BK + SwizzledLong<BK>(row, 2 * st + half) * 8);
+        } else {
+          // sixteen lanes read four of the depth by sixteen columns, and each gets one column's four
+          const int row = st * 16 + half * 8 + lane % 16 / 4, group = w_column(j) / 8 + lane / 16 % 2 * 2 + lane % 4 / 2;
+          uint16_t *const from = const_cast<uint16_t *>(w_from) + p * S::kWValues + row * BW + SwizzledWide(row, group) * 8 + lane % 2 * 4;
+          typedef __attribute__((address_space(3))) shortx4 *Lds;
+          const uint64_t first = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from)));
+          const uint64_t second = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + 4 * BW)));
+          o.w[j][p] = u32x4{static_cast<uint32_t>(first), static_cast<uint32_t>(first >> 32), static_cast<uint32_t>(second), static_cast<uint32_t>(second >> 32)};
         }
       }
+    }
 #pragma unroll
-      for (int j = 0; j < S::kWTiles; ++j) {
+    for (int i = 0; i < S::kRowTiles; ++i) {
+      const int row = (wm * S::kRowTiles + i) * 32 + own;
 #pragma unroll
-        for (int i = 0; i < S::kRowTiles; ++i) {
-          if constexpr (kParted) {
-            MfmaParts<3>(w[j], x[i], acc[i][j], low[i][j]);
-          } else {
-            acc[i][j] = Mfma32<E>(w[j][0], x[i][0], acc[i][j]);
-          }
-        }
-      }
+      for (int p = 0; p < kParts; ++p) o.x[i][p] = *reinterpret_cast<const u32x4 *>(x_from + p * S::kXValues + row * BK + SwizzledLong<BK>(row, 2 * st + half) * 8);
     }
   };
-
-  fetch(0, 0);
-  store(0, 0);
-  int stage = 0;
-  for (int32_t k0 = 0; k0 < a.depth; k0 += BK) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();  // the stage is there for all, and everyone is done with the one before
+  auto multiply = [&](int stage) __attribute__((always_inline)) {
+    constexpr int kSteps = BK / 16 / S::WK;
+    Operands o[2];
+    read(o[0], stage, 0);
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+      if (step + 1 < kSteps) read(o[(step + 1) % 2], stage, step + 1);
+      const Operands &now = o[step % 2];
+#pragma unroll
+      for (int i = 0; i < S::kRowTiles; ++i) {
+#pragma unroll
+        for (int j = 0; j < S::kWTiles; ++j) {
+          if constexpr (kParted) {
+            MfmaParts<3>(now.w[j], now.x[i], acc[i][j], low[i][j]);
+          } else {
+            acc[i][j] = Mfma32<E>(now.w[j][0], now.x[i][0], acc[i][j]);
+          }
+        }
+      }
+    }
+    if constexpr (!kParted && S::WK == 1) {
+      // the order asked for: a step's operands are read between the products of the step before
+      constexpr int kProducts = S::kRowTiles * S::kWTiles, kReads = S::kRowTiles + S::kWTiles * (ROWS ? 1 : 2);
+      __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+      StaticFor<kSteps>([&](auto step) __attribute__((always_inline)) {
+        constexpr int left = decltype(step)::value + 1 < kSteps ? kReads : 0, each = (left + kProducts - 1) / kProducts;
+        StaticFor<kProducts>([&](auto n) __attribute__((always_inline)) {
+          constexpr int some = left - decltype(n)::value * each < 0 ? 0 : left - decltype(n)::value * each < each ? left - decltype(n)::value * each : each;
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          if constexpr (some > 0) __builtin_amdgcn_sched_group_barrier(0x100, some, 0);
+        });
+      });
+    }
+  };
+  auto ready = [&]() __attribute__((always_inline)) {  // the stage is there for all, and everyone is done with the one before
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if constexpr (!kParted && S::kAhead == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const bool more = k0 + BK < a.depth;
-    if constexpr (S::kStages == 2) {
-      if (more) fetch(k0 + BK, stage ^ 1);
+  };
+
+  if constexpr (S::kAhead > 1) {
+    // few products to a stage: the time is that of the loads, so several stages are on their way
+    Held held[S::kAhead];
+    StaticFor<S::kAhead>([&](auto n) __attribute__((always_inline)) {
+      if (n * BK < a.depth) fetch(held[n], n * BK, true, true);
+    });
+    store(held[0], 0, true, true);
+    for (int32_t k0 = 0; k0 < a.depth; k0 += S::kAhead * BK) {
+      StaticFor<S::kAhead>([&](auto n) __attribute__((always_inline)) {
+        const int32_t k = k0 + n * BK;
+        if (k >= a.depth) return;
+        ready();
+        if (k + S::kAhead * BK < a.depth) fetch(held[n], k + S::kAhead * BK, true, true);
+        multiply(n % 2);
+        if (k + BK < a.depth) store(held[(n + 1) % S::kAhead], (n + 1) % 2, true, true);
+      });
+    }
+  } else {
+    Held held;
+    auto begin = [&](int32_t k0, int stage) __attribute__((always_inline)) {
+      const bool near = direct(k0);
+      fetch_direct(k0, stage, near && (S::kLarge || a.x_direct), near && (S::kLarge || a.weights_direct));
+      if constexpr (!S::kLarge) fetch(held, k0, !(near && a.x_direct), !(near && a.weights_direct));
+    };
+    auto end = [&](int32_t k0, int stage) __attribute__((always_inline)) {
+      const bool near = direct(k0);
+      if constexpr (!S::kLarge) store(held, stage, !(near && a.x_direct), !(near && a.weights_direct));
+    };
+    begin(0, 0);
+    end(0, 0);
+    int stage = 0;
+    for (int32_t k0 = 0; k0 < a.depth; k0 += BK) {
+      ready();
+      const bool more = k0 + BK < a.depth;
+      if (more) begin(k0 + BK, stage ^ 1);
       multiply(stage);
-      if (more) store(k0 + BK, stage ^ 1);
+      if (more) end(k0 + BK, stage ^ 1);
       stage ^= 1;
-    } else {
-      if (more) fetch(k0 + BK, 0);
-      multiply(0);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      if (more) store(k0 + BK, 0);
     }
   }
-  asm volatile("s_nop 15\ns_nop 3");  // (the last products, across the loop's branch: see Settle in attention_positions.hip)
+  SettleAcrossBranch();
 #pragma unroll
   for (int i = 0; i < S::kRowTiles; ++i) {
 #pragma unroll
@@ -371,7 +444,7 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::kThreads == 512 ? 2 : 1) vo
   }
 
   if constexpr (S::WK > 1) {  // the waves that share the depth: the first adds the others' sums, in their order
-    static_assert(S::WM == 1 && S::WN == 1 && S::kLds >= S::kRowTiles * S::kWTiles * 2 * kWave * 17, "sums fit");
+    static_assert(S::WM == 1 && S::WN == 1 && S::kAhead % 2 == 0 && S::kLds >= S::kRowTiles * S::kWTiles * 2 * kWave * 17, "sums fit");
     float *const sums = reinterpret_cast<float *>(lds);
     for (int w = 1; w < S::WK; ++w) {
       __syncthreads();
@@ -588,7 +661,7 @@ __global__ __launch_bounds__(512, 2) void GatedFewKernel(const GatedArgs a) {
     }
     multiply(r);
   }
-  asm volatile("s_nop 10");  // (the last products, across the loop's branch: see Settle in attention_positions.hip)
+  SettleAcrossBranch();
 #pragma unroll
   for (int c = 0; c < kTiles; ++c) {
     if (c > 0) __syncthreads();
@@ -675,7 +748,7 @@ int LaunchLayout(GatedArgs &a, hipStream_t stream) {
     if (tiles(128, 128) >= 256) return LaunchTiles<T, TileShape<T, 128, 128, 2, 2, 1, 32, GATED, ROWS>>(a, stream);
     return LaunchTiles<T, TileShape<T, 32, 64, 1, 1, 4, 64, GATED, ROWS>>(a, stream);
   } else {
-    if (tiles(256, 256) >= 200) return LaunchTiles<T, TileShape<T, 256, 256, 2, 4, 1, 64, GATED, ROWS>>(a, stream);
+    if (tiles(256, 256) >= 200 && a.x_direct && a.weights_direct && a.depth % 64 == 0) return LaunchTiles<T, TileShape<T, 256, 256, 2, 4, 1, 64, GATED, ROWS>>(a, stream);
     if (tiles(128, 128) >= 256) return LaunchTiles<T, TileShape<T, 128, 128, 2, 2, 1, 64, GATED, ROWS>>(a, stream);
     return LaunchTiles<T, TileShape<T, 64, 64, 1, 1, 4, 64, GATED, ROWS>>(a, stream);
   }
