@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Iterable, Optional, Sequence
 
 FL_MAX_RANK = 8
@@ -316,6 +317,9 @@ def make_tensor(base: int, dtype: int, shape: Sequence[int], strides: Optional[S
 
 _TORCH_DTYPES = {"torch.bool": FL_BOOL, "torch.int32": FL_INT32, "torch.int64": FL_INT64, "torch.float16": FL_FLOAT16,
                  "torch.bfloat16": FL_BFLOAT16, "torch.float32": FL_FLOAT32, "torch.float64": FL_FLOAT64}
+_DTYPE_OF = {}  # the same by the types themselves, as they are met (this module does not import torch)
+_HEAD = [struct.Struct(f"=Qii{n}q") for n in range(FL_MAX_RANK + 1)]
+_STRIDES = [struct.Struct(f"={n}q") for n in range(FL_MAX_RANK + 1)]
 
 
 def view(t) -> FlTensor:
@@ -323,7 +327,13 @@ def view(t) -> FlTensor:
     rank = t.dim()
     if rank > FL_MAX_RANK:
         raise ValueError(f"rank {rank} exceeds FL_MAX_RANK={FL_MAX_RANK}")
-    return FlTensor(t.data_ptr(), _TORCH_DTYPES[str(t.dtype)], rank, tuple(t.shape), t.stride())
+    dtype = _DTYPE_OF.get(t.dtype)
+    if dtype is None:
+        dtype = _DTYPE_OF[t.dtype] = _TORCH_DTYPES[str(t.dtype)]
+    v = FlTensor()
+    _HEAD[rank].pack_into(v, 0, t.data_ptr(), dtype, rank, *t.shape)
+    _STRIDES[rank].pack_into(v, FlTensor.strides.offset, *t.stride())
+    return v
 
 
 def i64_array(values: Iterable[int]):

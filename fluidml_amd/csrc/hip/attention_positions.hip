@@ -285,11 +285,15 @@ __device__ __forceinline__ void ReadAhead() {
   __builtin_amdgcn_sched_group_barrier(kProduct, AHEAD, 0);
 }
 
-// Eight neighbouring values of a row from column d on, zeros behind the last column.
+// Eight neighbouring values of a row from column d on, zeros behind the last column.  (No branch around a load: what is not there is read as the
+// last column.)
 template <typename T>
 __device__ __forceinline__ void Load8(const T *row, int64_t stride, int d, int columns, float (&x)[8]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = d + e < columns ? static_cast<float>(row[(d + e) * stride]) : 0.0f;
+  for (int e = 0; e < 8; ++e) {
+    const float v = static_cast<float>(row[min(d + e, columns - 1) * stride]);
+    x[e] = d + e < columns ? v : 0.0f;
+  }
 }
 
 // ... of a query, whose first of eight is there
@@ -1038,7 +1042,7 @@ constexpr int64_t kPartialBytes = 16 << 20;
 Plan MakePlan(const fl_tensor *q, const fl_tensor *k, const fl_attention_scores *s, bool aligned) {
   const int64_t B = q->shape[0], KV = k->shape[1], Skv = k->shape[2], D = q->shape[3], rows = q->shape[2] * (q->shape[1] / KV);
   Plan p{};
-  p.many = aligned && B * KV * ((rows + 127) / 128) >= 192;
+  p.many = aligned && rows > 32 && B * KV * ((rows + 127) / 128) >= 192;
   p.splits = 1;
   if (!p.many) {
     const int64_t tiles = B * KV * ((rows + 15) / 16);

@@ -15,8 +15,9 @@ struct GatedArgs {
   int32_t rows, depth, columns, activation;
   FastDiv row_tiles, column_tiles, group;  // tiles of x, of the weights; tiles of x that are walked together times those of the weights
   int32_t out_vectors;  // four results of a row in one store
-  int32_t x_direct, weights_direct;  // straight into LDS: 16-byte aligned, and near enough for 32-bit offsets
-  int32_t x_run, gate_run, up_run;   // values of the layout's long side lie side by side
+  int32_t x_near, weights_near;      // runs of whole words, near enough for 32-bit offsets ..
+  int32_t x_direct, weights_direct;  // .. and 16-byte aligned: straight into LDS
+  int32_t x_run, gate_run, up_run;   // values of the layout's long side lie side by side: 2 in whole words, 1 at any address, 0 not
 };
 
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
@@ -111,9 +112,10 @@ struct TileShape {
   static constexpr int kRowTiles = BM / WM / 32, kWTiles = BW / WN / 32;
   static constexpr int kXValues = BM * BK, kWValues = BW * BK;
   static constexpr int kStage = kParts * (kXValues + kWValues);
-  static constexpr int kLds = kStage * 2;
+  static constexpr int kBuffers = kParted ? 1 : 2;       // two workgroups of the one hide more than two buffers of one workgroup
+  static constexpr int kLds = kStage * kBuffers;
   static constexpr bool kLarge = BM == 256;             // direct loads only
-  static constexpr int kAhead = WK > 1 ? 4 : 1;         // stages on their way in registers
+  static constexpr int kAhead = WK > 1 || (kParted && BM < 128) ? 2 : 1;  // stages on their way in registers
   static_assert(kXGroups % kThreads == 0 && kWGroups % kThreads == 0 && BK % (16 * WK) == 0 && (!GATED || BW / WN == 64), "every thread and wave has the same to do");
 };
 
@@ -133,21 +135,75 @@ __device__ __forceinline__ floatx16 Mfma32(u32x4 x, u32x4 y, floatx16 acc) {
   }
 }
 
-// Eight values `stride` apart, the first `n` of which are there.
+// Values at .. at + 7 of a row whose values lie `stride` apart, zeros from `limit` on (which is at least 1).  No branch around a load: what is not
+// there is read as the last one.
 template <typename T>
 struct Eight {
   T v[8];
 };
 template <typename T>
-__device__ __forceinline__ Eight<T> LoadEight(const T *from, int64_t stride, int n) {
+__device__ __forceinline__ Eight<T> LoadEight(const T *row, int64_t stride, int32_t at, int32_t limit, bool there = true) {
   Eight<T> x;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x.v[e] = e < n ? from[e * stride] : static_cast<T>(0.0f);
+  for (int e = 0; e < 8; ++e) {
+    const T v = row[min(at + e, limit - 1) * stride];
+    x.v[e] = there && at + e < limit ? v : static_cast<T>(0.0f);
+  }
   return x;
 }
 
+// The same for values side by side at any address, `limit` at least N, without a branch around a load: the last N of the row where at + N > limit,
+// shifted.  16-bit values at odd addresses: whole words and the next one, turned (16 bytes at an odd address take the load three
+// times as long: 333 rows of 2731 by 1000 columns 65 us, of 2732 23).
+template <int N, typename T>
+struct Row {
+  typedef T Vec __attribute__((ext_vector_type(N)));
+  typedef uint32_t Words __attribute__((ext_vector_type(N * sizeof(T) / 4)));
+  typedef uint32_t LooseWords __attribute__((ext_vector_type(N * sizeof(T) / 4), aligned(4)));
+  static __device__ __forceinline__ Vec Load(const T *row, int32_t at, int32_t limit) {
+    const int32_t from = min(at, limit - N), shift = at - from;
+    Vec v, x;
+    if constexpr (sizeof(T) == 4) {
+      v = __builtin_bit_cast(Vec, Words(*reinterpret_cast<const LooseWords *>(row + from)));
+    } else {
+      constexpr int kWords = N / 2;
+      const uintptr_t where = reinterpret_cast<uintptr_t>(row + from);
+      const uint32_t odd = where & 2;
+      const uint32_t *const word = reinterpret_cast<const uint32_t *>(where - odd);
+      Words w = *reinterpret_cast<const LooseWords *>(word);
+      const uint32_t next = word[odd ? kWords : kWords - 1];  // (every word read holds a value of the row)
+#pragma unroll
+      for (int n = 0; n < kWords; ++n) w[n] = __builtin_amdgcn_alignbit(n + 1 < kWords ? w[(n + 1) % kWords] : next, w[n], odd * 8);
+      v = __builtin_bit_cast(Vec, w);
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        x[e] = static_cast<T>(0.0f);
+#pragma unroll
+        for (int n = e; n < N; ++n) x[e] = shift == n - e ? v[n] : x[e];
+      }
+    } else {
+      typedef uint64_t Longs __attribute__((ext_vector_type(N / 4)));
+      Longs w = __builtin_bit_cast(Longs, v);
+      const int bits = 16 * (shift & 3);
+      if constexpr (N == 8) {
+        const uint64_t low = shift < 4 ? w[0] : w[1], high = shift < 4 ? w[1] : 0;
+        w[0] = low >> bits | (bits == 0 ? 0 : high << (64 - bits));
+        w[1] = high >> bits;
+      } else {
+        w[0] >>= bits;
+      }
+      x = __builtin_bit_cast(Vec, w);
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[e] = shift < N ? x[e] : static_cast<T>(0.0f);
+    }
+    return x;
+  }
+};
+
 template <typename T, typename Shape>
-__global__ __launch_bounds__(Shape::kThreads, Shape::kThreads == 512 ? 2 : 1) void GatedTileKernel(const GatedArgs a) {
+__global__ __launch_bounds__(Shape::kThreads, Shape::WK > 2 ? 3 : 2) void GatedTileKernel(const GatedArgs a) {
   using S = Shape;
   constexpr int BK = S::BK, BW = S::BW, BN = S::BN, kParts = S::kParts;
   constexpr bool kParted = S::kParted, GATED = S::GATED, ROWS = S::ROWS;
@@ -174,31 +230,39 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::kThreads == 512 ? 2 : 1) vo
   const T *const up_tile = GATED ? static_cast<const T *>(a.up) + n0 * a.up_strides[1] : nullptr;
 
   // where a thread's groups come from.  x: row and group of the depth.  Weights: column and group of the depth (ROWS), or depth and group of columns
-  uint32_t x_offset[kParted ? 1 : S::kXLoads], w_offset[kParted ? 1 : S::kWLoads];
-  if constexpr (!kParted) {
+  uint32_t x_offset[S::kXLoads], w_offset[S::kWLoads];  // bytes, where 32 bits hold them
+  constexpr uint32_t kItem = sizeof(T);
 #pragma unroll
-    for (int n = 0; n < S::kXLoads; ++n) {
-      const int place = (wave * S::kXLoads + n) * kWave + lane, row = place / (BK / 8), group = SwizzledLong<BK>(row, place % (BK / 8));
-      x_offset[n] = static_cast<uint32_t>(min(row, a.rows - 1 - m0)) * static_cast<uint32_t>(a.x_strides[0]) * 2 + group * 16;
-    }
+  for (int n = 0; n < S::kXLoads; ++n) {
+    const int place = (wave * S::kXLoads + n) * kWave + lane, row = place / (BK / 8), group = SwizzledLong<BK>(row, place % (BK / 8));
+    x_offset[n] = (static_cast<uint32_t>(min(row, a.rows - 1 - m0)) * static_cast<uint32_t>(a.x_strides[0]) + group * 8) * kItem;
+  }
 #pragma unroll
-    for (int n = 0; n < S::kWLoads; ++n) {
-      const int place = (wave * S::kWLoads + n) * kWave + lane;
-      if constexpr (ROWS) {
-        const int row = place / (BK / 8), group = SwizzledLong<BK>(row, place % (BK / 8));
-        const bool up = GATED && row >= BN;
-        w_offset[n] = static_cast<uint32_t>(min(up ? row - BN : row, a.columns - 1 - n0)) * static_cast<uint32_t>(up ? a.up_strides[1] : a.gate_strides[1]) * 2 + group * 16;
-      } else {
-        const int row = place / (BW / 8), group = SwizzledWide(row, place % (BW / 8));
-        const bool up = GATED && group >= BN / 8;
-        // (columns behind the last: the last group again, whose results are not stored)
-        w_offset[n] = static_cast<uint32_t>(row) * static_cast<uint32_t>(up ? a.up_strides[0] : a.gate_strides[0]) * 2 +
-                      min(up ? group - BN / 8 : group, (a.columns - 1 - n0) / 8) * 16;
-      }
+  for (int n = 0; n < S::kWLoads; ++n) {
+    const int place = (wave * S::kWLoads + n) * kWave + lane;
+    if constexpr (ROWS) {
+      const int row = place / (BK / 8), group = SwizzledLong<BK>(row, place % (BK / 8));
+      const bool up = GATED && row >= BN;
+      w_offset[n] = (static_cast<uint32_t>(min(up ? row - BN : row, a.columns - 1 - n0)) * static_cast<uint32_t>(up ? a.up_strides[1] : a.gate_strides[1]) + group * 8) * kItem;
+    } else {
+      const int row = place / (BW / 8), group = SwizzledWide(row, place % (BW / 8));
+      const bool up = GATED && group >= BN / 8;
+      // (columns behind the last: the last group again, whose results are not stored)
+      w_offset[n] = (static_cast<uint32_t>(row) * static_cast<uint32_t>(up ? a.up_strides[0] : a.gate_strides[0]) +
+                     min(up ? group - BN / 8 : group, (a.columns - 1 - n0) / 8) * 8) * kItem;
     }
   }
   // (a group is the gate's or the up projection's by its place alone: the same for a whole load of a wave where ROWS, else by lane)
   auto direct = [&](int32_t k0) __attribute__((always_inline)) { return S::kLarge || (!kParted && S::kAhead == 1 && k0 + BK <= a.depth); };
+  auto weights_from = [&](int32_t k0, int n) __attribute__((always_inline)) {
+    const T *from = gate_tile + (ROWS ? k0 : k0 * a.gate_strides[0]);
+    if constexpr (GATED) {
+      const int place = (wave * S::kWLoads + n) * kWave + lane;
+      const bool up = ROWS ? (wave * S::kWLoads + n) * kWave / (BK / 8) >= BN : SwizzledWide(place / (BW / 8), place % (BW / 8)) >= BN / 8;
+      if (up) from = up_tile + (ROWS ? k0 : k0 * a.up_strides[0]);
+    }
+    return reinterpret_cast<const char *>(from) + w_offset[n];
+  };
   auto fetch_direct = [&](int32_t k0, int stage, bool x, bool weights) __attribute__((always_inline)) {
     if constexpr (!kParted) {
       uint16_t *const x_to = lds + stage * S::kStage, *const w_to = x_to + kParts * S::kXValues;
@@ -208,19 +272,8 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::kThreads == 512 ? 2 : 1) vo
         for (int n = 0; n < S::kXLoads; ++n) LoadToLds(from + x_offset[n], x_to + (wave * S::kXLoads + n) * kWave * 8);
       }
       if (weights) {
-        const int64_t step = ROWS ? 1 : a.gate_strides[0], up_step = ROWS ? 1 : a.up_strides[0];
-        const char *const gate = reinterpret_cast<const char *>(gate_tile + k0 * step), *const up = reinterpret_cast<const char *>(up_tile + (GATED ? k0 * up_step : 0));
 #pragma unroll
-        for (int n = 0; n < S::kWLoads; ++n) {
-          const int place = (wave * S::kWLoads + n) * kWave + lane;
-          const char *from = gate;
-          if constexpr (GATED && ROWS) {
-            if ((wave * S::kWLoads + n) * kWave / (BK / 8) >= BN) from = up;
-          } else if constexpr (GATED) {
-            if (SwizzledWide(place / (BW / 8), place % (BW / 8)) >= BN / 8) from = up;
-          }
-          LoadToLds(from + w_offset[n], w_to + (wave * S::kWLoads + n) * kWave * 8);
-        }
+        for (int n = 0; n < S::kWLoads; ++n) LoadToLds(weights_from(k0, n), w_to + (wave * S::kWLoads + n) * kWave * 8);
       }
     }
   };
@@ -231,52 +284,50 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::kThreads == 512 ? 2 : 1) vo
   auto fetch = [&](Held &held, int32_t k0, bool x, bool weights) __attribute__((always_inline)) {
     const bool whole = k0 + BK <= a.depth;
     if (x) {
-      auto at = [&](int n, int32_t &k) __attribute__((always_inline)) {
-        const int place = (wave * S::kXLoads + n) * kWave + lane, row = place / (BK / 8), group = SwizzledLong<BK>(row, place % (BK / 8));
-        k = k0 + group * 8;
-        return x_tile + min(row, a.rows - 1 - m0) * a.x_strides[0] + k * a.x_strides[1];
-      };
-      int32_t k;
-      if (whole && a.x_run) {
 #pragma unroll
-        for (int n = 0; n < S::kXLoads; ++n) __builtin_memcpy(&held.x[n], at(n, k), sizeof(Eight<T>));
-      } else {
-#pragma unroll
-        for (int n = 0; n < S::kXLoads; ++n) {
-          const T *const from = at(n, k);
-          held.x[n] = LoadEight<T>(from, a.x_strides[1], a.depth - k);
+      for (int n = 0; n < S::kXLoads; ++n) {
+        const int place = (wave * S::kXLoads + n) * kWave + lane, row = place / (BK / 8), k = k0 + SwizzledLong<BK>(row, place % (BK / 8)) * 8;
+        const T *const from = x_tile + min(row, a.rows - 1 - m0) * a.x_strides[0];
+        if (whole && a.x_near) {
+          __builtin_memcpy(&held.x[n], __builtin_assume_aligned(reinterpret_cast<const char *>(x_tile + k0) + x_offset[n], 4), sizeof(Eight<T>));
+        } else if (a.x_run && a.depth >= 8) {
+          held.x[n] = __builtin_bit_cast(Eight<T>, Row<8, T>::Load(from, k, a.depth));
+        } else {
+          held.x[n] = LoadEight<T>(from, a.x_strides[1], k, a.depth);
         }
       }
     }
     if (weights) {
-      // `there`: values of the group that are
-      auto at = [&](int n, int64_t &stride, int32_t &there) __attribute__((always_inline)) {
+      const bool runs = a.gate_run && (!GATED || a.up_run), run = a.weights_near && whole && (ROWS || n0 + BN <= a.columns);
+#pragma unroll
+      for (int n = 0; n < S::kWLoads; ++n) {
         const int place = (wave * S::kWLoads + n) * kWave + lane;
         const int row = ROWS ? place / (BK / 8) : place / (BW / 8);
         const int group = ROWS ? SwizzledLong<BK>(row, place % (BK / 8)) : SwizzledWide(row, place % (BW / 8));
         const bool up = GATED && (ROWS ? row >= BN : group >= BN / 8);
         const int64_t along = up ? a.up_strides[0] : a.gate_strides[0], across = up ? a.up_strides[1] : a.gate_strides[1];
-        const T *const from = up ? up_tile : gate_tile;
+        const T *from = up ? up_tile : gate_tile;
         if constexpr (ROWS) {
           const int32_t k = k0 + group * 8;
-          stride = along, there = a.depth - k;
-          return from + min(up ? row - BN : row, a.columns - 1 - n0) * across + k * along;
+          from += min(up ? row - BN : row, a.columns - 1 - n0) * across;
+          if (run) {
+            __builtin_memcpy(&held.w[n], __builtin_assume_aligned(weights_from(k0, n), 4), sizeof(Eight<T>));
+          } else if (runs && a.depth >= 8) {
+            held.w[n] = __builtin_bit_cast(Eight<T>, Row<8, T>::Load(from, k, a.depth));
+          } else {
+            held.w[n] = LoadEight<T>(from, along, k, a.depth);
+          }
         } else {
           const int32_t k = k0 + row, c = (up ? group - BN / 8 : group) * 8;
-          stride = across, there = k < a.depth ? a.columns - n0 - c : 0;
-          return from + c * across + k * along;
-        }
-      };
-      int64_t stride;
-      int32_t there;
-      if (whole && a.gate_run && (!GATED || a.up_run) && (ROWS || n0 + BN <= a.columns)) {
-#pragma unroll
-        for (int n = 0; n < S::kWLoads; ++n) __builtin_memcpy(&held.w[n], at(n, stride, there), sizeof(Eight<T>));
-      } else {
-#pragma unroll
-        for (int n = 0; n < S::kWLoads; ++n) {
-          const T *const from = at(n, stride, there);
-          held.w[n] = LoadEight<T>(from, stride, there);
+          from += min(k, a.depth - 1) * along;
+          if (run) {
+            __builtin_memcpy(&held.w[n], __builtin_assume_aligned(weights_from(k0, n), 4), sizeof(Eight<T>));
+          } else if (runs && a.columns - n0 >= 8) {
+            held.w[n] = __builtin_bit_cast(Eight<T>, Row<8, T>::Load(from, c, k < a.depth ? a.columns - n0 : 8));
+            if (k >= a.depth) held.w[n] = Eight<T>{};
+          } else {
+            held.w[n] = LoadEight<T>(from, across, c, a.columns - n0, k < a.depth);
+          }
         }
       }
     }
@@ -349,13 +400,17 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::kThreads == 512 ? 2 : 1) vo
     }
   };
   auto multiply = [&](int stage) __attribute__((always_inline)) {
-    constexpr int kSteps = BK / 16 / S::WK;
-    Operands o[2];
-    read(o[0], stage, 0);
+    constexpr int kSteps = BK / 16 / S::WK, kSets = kParted ? 1 : 2;
+    Operands o[kSets];
+    if constexpr (!kParted) read(o[0], stage, 0);
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      if (step + 1 < kSteps) read(o[(step + 1) % 2], stage, step + 1);
-      const Operands &now = o[step % 2];
+      if constexpr (kParted) {
+        read(o[0], stage, step);
+      } else {
+        if (step + 1 < kSteps) read(o[(step + 1) % kSets], stage, step + 1);
+      }
+      const Operands &now = o[step % kSets];
 #pragma unroll
       for (int i = 0; i < S::kRowTiles; ++i) {
 #pragma unroll
@@ -389,7 +444,23 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::kThreads == 512 ? 2 : 1) vo
     asm volatile("" ::: "memory");
   };
 
-  if constexpr (S::kAhead > 1) {
+  if constexpr (kParted) {
+    Held held[S::kAhead];
+    StaticFor<S::kAhead>([&](auto n) __attribute__((always_inline)) {
+      if (n * BK < a.depth) fetch(held[n], n * BK, true, true);
+    });
+    for (int32_t k0 = 0; k0 < a.depth; k0 += S::kAhead * BK) {
+      StaticFor<S::kAhead>([&](auto n) __attribute__((always_inline)) {
+        const int32_t k = k0 + n * BK;
+        if (k >= a.depth) return;
+        ready();
+        store(held[n], 0, true, true);
+        if (k + S::kAhead * BK < a.depth) fetch(held[n], k + S::kAhead * BK, true, true);
+        ready();
+        multiply(0);
+      });
+    }
+  } else if constexpr (S::kAhead > 1) {
     // few products to a stage: the time is that of the loads, so several stages are on their way
     Held held[S::kAhead];
     StaticFor<S::kAhead>([&](auto n) __attribute__((always_inline)) {
@@ -444,8 +515,9 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::kThreads == 512 ? 2 : 1) vo
   }
 
   if constexpr (S::WK > 1) {  // the waves that share the depth: the first adds the others' sums, in their order
-    static_assert(S::WM == 1 && S::WN == 1 && S::kAhead % 2 == 0 && S::kLds >= S::kRowTiles * S::kWTiles * 2 * kWave * 17, "sums fit");
-    float *const sums = reinterpret_cast<float *>(lds);
+    constexpr int kSums = S::kRowTiles * S::kWTiles * 16 * kWave;
+    static_assert(S::kLds >= S::WM * S::WN * kSums * 2, "sums fit");
+    float *const sums = reinterpret_cast<float *>(lds) + wave / S::WK * kSums;
     for (int w = 1; w < S::WK; ++w) {
       __syncthreads();
       if (wk == w) {
@@ -535,23 +607,29 @@ __global__ __launch_bounds__(512, 2) void GatedFewKernel(const GatedArgs a) {
   constexpr int RT = S::RT, kMatrices = S::kMatrices, kGroup = S::kGroup, kSteps = S::kSteps, kTiles = S::kTiles;
   typedef T Group __attribute__((ext_vector_type(kGroup)));
   typedef T Four __attribute__((ext_vector_type(4)));
-  typedef T Loose __attribute__((ext_vector_type(kGroup), aligned(sizeof(T))));   // at any address
-  typedef T LooseFour __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  typedef T Loose __attribute__((ext_vector_type(kGroup), aligned(4)));   // at any word
+  typedef T LooseFour __attribute__((ext_vector_type(4), aligned(4)));
   __shared__ float joined[S::kWaves][kMatrices][RT][256];
   const int lane = threadIdx.x % kWave, own = lane % 16, quarter = lane / 16, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int32_t n0 = static_cast<int32_t>(blockIdx.x) * S::kColumns;
+  // (the tiles of rows of the same columns one after the other on one XCD, which has the weights then)
+  uint32_t id = blockIdx.x;
+  const uint32_t total = a.row_tiles.divisor * a.column_tiles.divisor, even = total / 8 * 8;
+  if (id < even) id = id % 8 * (total / 8) + id / 8;
+  const uint32_t column_tile = a.row_tiles.Div(id);
+  const int32_t n0 = static_cast<int32_t>(column_tile) * S::kColumns, m0 = static_cast<int32_t>(id - column_tile * a.row_tiles.divisor) * RT * 16;
   const T *const x_own = static_cast<const T *>(a.x);
   const T *const matrix[2] = {static_cast<const T *>(a.gate), static_cast<const T *>(GATED ? a.up : a.gate)};
   const int64_t along[2] = {a.gate_strides[0], a.up_strides[0]}, across[2] = {a.gate_strides[1], a.up_strides[1]};
-  const bool runs = a.x_run && a.gate_run && (!GATED || a.up_run) && (ROWS || n0 + S::kColumns <= a.columns);
 
   struct Run {
     Group x[kSteps][RT];
     Group w[ROWS ? kMatrices : 1][ROWS ? kSteps : 1];
     Four v[ROWS ? 1 : kMatrices][ROWS ? 1 : kSteps][ROWS ? 1 : kGroup];  // [depth][columns]
   };
+  const bool runs = a.x_run && a.gate_run && (!GATED || a.up_run) && a.depth >= kGroup && (ROWS || a.columns >= 4);
+  const bool inside = (ROWS || n0 + S::kColumns <= a.columns) && a.x_run == 2 && a.gate_run == 2 && (!GATED || a.up_run == 2);
   auto load = [&](Run &r, int32_t k0) __attribute__((always_inline)) {
-    if (runs && k0 + S::kDepth <= a.depth) {
+    if (inside && k0 + S::kDepth <= a.depth) {
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const int32_t k = k0 + s * S::kStep + quarter * kGroup;
@@ -565,9 +643,28 @@ __global__ __launch_bounds__(512, 2) void GatedFewKernel(const GatedArgs a) {
           }
         }
 #pragma unroll
-        for (int t = 0; t < RT; ++t) r.x[s][t] = *reinterpret_cast<const Loose *>(x_own + min(t * 16 + own, a.rows - 1) * a.x_strides[0] + k);
+        for (int t = 0; t < RT; ++t) r.x[s][t] = *reinterpret_cast<const Loose *>(x_own + min(m0 + t * 16 + own, a.rows - 1) * a.x_strides[0] + k);
       }
-    } else {  // value by value, zeros behind the ends
+    } else if (runs) {  // the same at the ends, and at odd addresses
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int32_t k = k0 + s * S::kStep + quarter * kGroup;
+#pragma unroll
+        for (int m = 0; m < kMatrices; ++m) {
+          if constexpr (ROWS) {
+            r.w[m][s] = Row<kGroup, T>::Load(matrix[m] + min(n0 + own, a.columns - 1) * across[m], k, a.depth);
+          } else {
+#pragma unroll
+            for (int e = 0; e < kGroup; ++e) {
+              const Four v = Row<4, T>::Load(matrix[m] + min(k + e, a.depth - 1) * along[m], n0 + own * 4, a.columns);
+              r.v[m][s][e] = k + e < a.depth ? v : Four{};
+            }
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t) r.x[s][t] = Row<kGroup, T>::Load(x_own + min(m0 + t * 16 + own, a.rows - 1) * a.x_strides[0], k, a.depth);
+      }
+    } else {  // value by value, zeros behind the ends (no branch around a load)
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const int32_t k = k0 + s * S::kStep + quarter * kGroup;
@@ -576,23 +673,30 @@ __global__ __launch_bounds__(512, 2) void GatedFewKernel(const GatedArgs a) {
           if constexpr (ROWS) {
             const T *const from = matrix[m] + min(n0 + own, a.columns - 1) * across[m];
 #pragma unroll
-            for (int e = 0; e < kGroup; ++e) r.w[m][s][e] = k + e < a.depth ? from[(k + e) * along[m]] : static_cast<T>(0.0f);
+            for (int e = 0; e < kGroup; ++e) {
+              const T v = from[min(k + e, a.depth - 1) * along[m]];
+              r.w[m][s][e] = k + e < a.depth ? v : static_cast<T>(0.0f);
+            }
           } else {
 #pragma unroll
             for (int e = 0; e < kGroup; ++e) {
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
                 const int32_t n = n0 + own * 4 + c;
-                r.v[m][s][e][c] = k + e < a.depth && n < a.columns ? matrix[m][(k + e) * along[m] + n * across[m]] : static_cast<T>(0.0f);
+                const T v = matrix[m][min(k + e, a.depth - 1) * along[m] + min(n, a.columns - 1) * across[m]];
+                r.v[m][s][e][c] = k + e < a.depth && n < a.columns ? v : static_cast<T>(0.0f);
               }
             }
           }
         }
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-          const T *const from = x_own + min(t * 16 + own, a.rows - 1) * a.x_strides[0];
+          const T *const from = x_own + min(m0 + t * 16 + own, a.rows - 1) * a.x_strides[0];
 #pragma unroll
-          for (int e = 0; e < kGroup; ++e) r.x[s][t][e] = k + e < a.depth ? from[(k + e) * a.x_strides[1]] : static_cast<T>(0.0f);
+          for (int e = 0; e < kGroup; ++e) {
+            const T v = from[min(k + e, a.depth - 1) * a.x_strides[1]];
+            r.x[s][t][e] = k + e < a.depth ? v : static_cast<T>(0.0f);
+          }
         }
       }
     }
@@ -677,7 +781,7 @@ __global__ __launch_bounds__(512, 2) void GatedFewKernel(const GatedArgs a) {
     for (int at = threadIdx.x; at < RT * 256; at += 512) {
       // row `row` of x by column `place` of the tile: register place % 4 of lane (place / 4) * 16 + row
       const int t = at / 256, row = at % 256 / 16, place = at % 16, from = ((place / 4) * 16 + row) * 4 + place % 4;
-      const int32_t m = t * 16 + row, n = n0 + (ROWS ? place : place * 4 + c);
+      const int32_t m = m0 + t * 16 + row, n = n0 + (ROWS ? place : place * 4 + c);
       if (m >= a.rows || n >= a.columns) continue;
       float g = 0.0f, u = 0.0f;
 #pragma unroll
@@ -717,9 +821,9 @@ void Set(const fl_tensor *t, int64_t (&strides)[2]) {
   for (int i = 0; i < 2; ++i) strides[i] = t == nullptr ? 0 : t->strides[i];
 }
 
-bool Aligned(const fl_tensor *t, int unit) {
-  const int64_t group = static_cast<int64_t>(16 / (t->dtype == FL_FLOAT32 ? 4 : 2));
-  return IsAligned(t->base, 16) && t->strides[unit] == 1 && t->strides[1 - unit] % group == 0 && t->strides[1 - unit] < (1 << 22);
+int Run(const fl_tensor *t, int unit) {
+  if (t->strides[unit] != 1) return 0;
+  return t->dtype == FL_FLOAT32 || (IsAligned(t->base, 4) && (t->strides[1 - unit] % 2 == 0 || t->shape[1 - unit] == 1)) ? 2 : 1;
 }
 
 template <typename T, typename Shape>
@@ -734,24 +838,32 @@ int LaunchTiles(GatedArgs &a, hipStream_t stream) {
 }
 
 template <typename T, typename Shape>
-int LaunchFew(const GatedArgs &a, hipStream_t stream) {
-  FL_LAUNCH((GatedFewKernel<T, Shape>), dim3((a.columns + Shape::kColumns - 1) / Shape::kColumns), dim3(512), 0, stream, a);
+int LaunchFew(GatedArgs &a, hipStream_t stream) {
+  const int64_t rows = (a.rows + Shape::RT * 16 - 1) / (Shape::RT * 16), columns = (a.columns + Shape::kColumns - 1) / Shape::kColumns;
+  if (rows * columns > INT32_MAX / 16) return FL_ERR_TOO_LARGE;
+  a.row_tiles = FastDiv(static_cast<uint32_t>(rows));
+  a.column_tiles = FastDiv(static_cast<uint32_t>(columns));
+  FL_LAUNCH((GatedFewKernel<T, Shape>), dim3(static_cast<uint32_t>(rows * columns)), dim3(512), 0, stream, a);
   return LaunchStatus();
 }
 
 template <typename T, bool GATED, bool ROWS>
 int LaunchLayout(GatedArgs &a, hipStream_t stream) {
+  auto tiles = [&](int64_t bm, int64_t bw) { return (a.rows + bm - 1) / bm * ((a.columns + bw / (GATED ? 2 : 1) - 1) / (bw / (GATED ? 2 : 1))); };
   if (a.rows <= 16) return LaunchFew<T, FewShape<T, GATED, ROWS, 1>>(a, stream);
   if (a.rows <= 32) return LaunchFew<T, FewShape<T, GATED, ROWS, 2>>(a, stream);
-  auto tiles = [&](int64_t bm, int64_t bw) { return (a.rows + bm - 1) / bm * ((a.columns + bw / (GATED ? 2 : 1) - 1) / (bw / (GATED ? 2 : 1))); };
   if constexpr (std::is_same_v<T, float>) {
     if (tiles(128, 128) >= 256) return LaunchTiles<T, TileShape<T, 128, 128, 2, 2, 1, 32, GATED, ROWS>>(a, stream);
-    return LaunchTiles<T, TileShape<T, 32, 64, 1, 1, 4, 64, GATED, ROWS>>(a, stream);
+    if (tiles(64, 128) >= 128) return LaunchTiles<T, TileShape<T, 64, 128, 2, 2, 2, 64, GATED, ROWS>>(a, stream);
   } else {
     if (tiles(256, 256) >= 200 && a.x_direct && a.weights_direct && a.depth % 64 == 0) return LaunchTiles<T, TileShape<T, 256, 256, 2, 4, 1, 64, GATED, ROWS>>(a, stream);
-    if (tiles(128, 128) >= 256) return LaunchTiles<T, TileShape<T, 128, 128, 2, 2, 1, 64, GATED, ROWS>>(a, stream);
-    return LaunchTiles<T, TileShape<T, 64, 64, 1, 1, 4, 64, GATED, ROWS>>(a, stream);
+    if (tiles(128, 128) >= 128) return LaunchTiles<T, TileShape<T, 128, 128, 2, 2, 1, 64, GATED, ROWS>>(a, stream);
+    if (tiles(64, 64) >= 256) return LaunchTiles<T, TileShape<T, 64, 64, 1, 1, 4, 64, GATED, ROWS>>(a, stream);
   }
+  // few tiles: sixteen rows a workgroup where thirty-two leave compute units without one
+  constexpr int kColumns = FewShape<T, GATED, ROWS, 1>::kColumns;
+  if ((a.rows + 31) / 32 * ((a.columns + kColumns - 1) / kColumns) < 256) return LaunchFew<T, FewShape<T, GATED, ROWS, 1>>(a, stream);
+  return LaunchFew<T, FewShape<T, GATED, ROWS, 2>>(a, stream);
 }
 
 // out = act(x . gate + gate_bias) * (x . up + up_bias), or with `up` NULL: x . gate + gate_bias + addend
@@ -771,11 +883,16 @@ int Contract(const fl_tensor *x, const fl_tensor *gate, const fl_tensor *up, con
   // the layout that the weights share, or that of a checkpoint; a matrix that has another is read value by value
   const bool wide = gate->strides[1] == 1 && (up == nullptr || up->strides[1] == 1) && !(gate->strides[0] == 1 && gate->shape[1] > 1 && gate->shape[0] == 1);
   const int unit = wide ? 1 : 0;
-  a.x_direct = Aligned(x, 1);
-  a.weights_direct = Aligned(gate, unit) && (up == nullptr || Aligned(up, unit)) && (!wide || a.columns % 8 == 0);
-  a.x_run = x->strides[1] == 1;
-  a.gate_run = gate->strides[unit] == 1;
-  a.up_run = up != nullptr && up->strides[unit] == 1;
+  a.x_run = Run(x, 1);
+  a.gate_run = Run(gate, unit);
+  a.up_run = up == nullptr ? 0 : Run(up, unit);
+  auto near = [](const fl_tensor *t, int u) { return Run(t, u) == 2 && t->strides[1 - u] < (1 << 21); };
+  const int64_t group = x->dtype == FL_FLOAT32 ? 4 : 8;
+  auto aligned = [&](const fl_tensor *t, int u) { return near(t, u) && IsAligned(t->base, 16) && t->strides[1 - u] % group == 0; };
+  a.x_near = near(x, 1);
+  a.weights_near = near(gate, unit) && (up == nullptr || near(up, unit));
+  a.x_direct = aligned(x, 1);
+  a.weights_direct = aligned(gate, unit) && (up == nullptr || aligned(up, unit)) && (!wide || a.columns % 8 == 0);
   const size_t item = x->dtype == FL_FLOAT32 ? 4 : 2;
   a.out_vectors = out->strides[1] == 1 && out->strides[0] % 4 == 0 && a.columns % 4 == 0 && IsAligned(out->base, 4 * item);
   return ForDecoderType(x->dtype, [&](auto type) {
