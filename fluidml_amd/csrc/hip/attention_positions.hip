@@ -326,7 +326,12 @@ struct RowsShape {
   static constexpr int kBuffers = PARTED ? 1 : 2;
   static constexpr int kPlane = BK * DP;                       // values of one part of a tile
   static constexpr int kValues = kBuffers * 2 * kParts * kPlane;  // of K and V
-  static constexpr int kSwizzleK = DP / 8 % 8 == 0 ? 7 : 3, kSwizzleV = DP / 8 % 8 == 0 ? 6 : 2;
+  // LDS serves 256 bytes at a time: sixteen lanes' 16 bytes of one column group of sixteen keys of K, 64 bytes of four keys of V.  A group of a
+  // row lies in the place whose number is its own, turned so that those fall on different banks, however many rows lie in 256 bytes.
+  static constexpr int kTurns = DP % 128 == 0 ? 16 : DP == 64 ? 8 : 4;  // K: places that a row's number chooses from
+  static constexpr int kVTurns = DP % 128 == 0 ? 4 : DP == 64 ? 2 : 1;  // V: in fours
+  static __host__ __device__ __forceinline__ constexpr int TurnK(int key) { return DP % 128 == 0 ? key & 15 : DP == 64 ? key >> 1 & 7 : key >> 2 & 3; }
+  static __host__ __device__ __forceinline__ constexpr int TurnV(int key) { return DP % 128 == 0 ? (key & 3) * 4 : DP == 64 ? (key >> 1 & 1) * 4 : 0; }
   static constexpr int kGroups = BK * DP / 8;                  // of eight values
   static constexpr int kLoads = kGroups / 256;                 // a thread's, per matrix
 };
@@ -429,7 +434,7 @@ __global__ __launch_bounds__(256, WAVES) void AttentionRowsKernel(const Attentio
 #pragma unroll
       for (int n = 0; n < Shape::kLoads; ++n) {
         const int place = (wave * Shape::kLoads + n) * kWave + lane, key = place / (DP / 8);
-        const int group = place % (DP / 8) ^ (m == 0 ? key & Shape::kSwizzleK : 2 * key & Shape::kSwizzleV);
+        const int group = place % (DP / 8) ^ (m == 0 ? Shape::TurnK(key) : Shape::TurnV(key));
         offset[m][n] = static_cast<uint32_t>(key) * static_cast<uint32_t>(m == 0 ? a.k.strides[2] : a.v.strides[2]) * 2 + min(group, last_group) * 16;
       }
     }
@@ -456,7 +461,7 @@ __global__ __launch_bounds__(256, WAVES) void AttentionRowsKernel(const Attentio
 #pragma unroll
       for (int n = 0; n < Shape::kLoads; ++n) {
         const int place = (wave * Shape::kLoads + n) * kWave + lane, key = place / (DP / 8);
-        const int group = place % (DP / 8) ^ (m == 0 ? key & Shape::kSwizzleK : 2 * key & Shape::kSwizzleV);
+        const int group = place % (DP / 8) ^ (m == 0 ? Shape::TurnK(key) : Shape::TurnV(key));
         // (columns behind the last and keys behind the last are read as the last: Q is zero there, and the weight of such a key)
         const T *const at = from + min(t * BK + key, seq.n_keys - 1) * stride + min(group, last_group) * 8;
         if constexpr (kParted) {
@@ -498,7 +503,7 @@ __global__ __launch_bounds__(256, WAVES) void AttentionRowsKernel(const Attentio
 
   const int k_row = lane % 32 * DP;                                            // K: key lane % 32 ..
   const int v_key = 4 * half + lane % 16 / 4;                                  // V: key ..
-  const int v_group = lane / 16 % 2 * 2 + lane % 4 / 2, v_swizzle = 2 * (lane % 16 / 4) & Shape::kSwizzleV;
+  const int v_group = lane / 16 % 2 * 2 + lane % 4 / 2, v_swizzle = Shape::TurnV(lane % 16 / 4);
 
   int32_t now_document = -1, next_document = -1, now = tiles.Next(a, b, now_document);
   int buffer = 0;
@@ -524,20 +529,30 @@ __global__ __launch_bounds__(256, WAVES) void AttentionRowsKernel(const Attentio
       floatx16 dots[kKeyTiles], lows[kParted ? kKeyTiles : 1];
 #pragma unroll
       for (int t = 0; t < kKeyTiles; ++t) {
-        floatx16 &dot = dots[t], &low = lows[kParted ? t : 0];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) dot[e] = 0.0f, low[e] = 0.0f;
+        for (int e = 0; e < 16; ++e) dots[t][e] = 0.0f, lows[kParted ? t : 0][e] = 0.0f;
+      }
+      // (neighbouring products go to different sums: one that waits for the one before it leaves the matrix pipe idle)
 #pragma unroll
-        for (int st = 0; st < kSteps; ++st) {
-          const int at = t * 32 * DP + k_row + ((2 * st + half) ^ (lane & Shape::kSwizzleK)) * 8;
-          u32x4 k[kParts];
+      for (int st = 0; st < kSteps; ++st) {
+        u32x4 k[kKeyTiles][kParts];
 #pragma unroll
-          for (int p = 0; p < kParts; ++p) k[p] = *reinterpret_cast<const u32x4 *>(k_tile + p * Shape::kPlane + at);
-          if constexpr (kParted) {
-            MfmaParts<3>(k, q[st], dot, low);
-          } else {
-            dot = Mfma32<E>(k[0], q[st][0], dot);
-          }
+        for (int t = 0; t < kKeyTiles; ++t) {
+          const int at = t * 32 * DP + k_row + ((2 * st + half) ^ Shape::TurnK(lane % 32)) * 8;
+#pragma unroll
+          for (int p = 0; p < kParts; ++p) k[t][p] = *reinterpret_cast<const u32x4 *>(k_tile + p * Shape::kPlane + at);
+        }
+        if constexpr (kParted) {
+          ForParts([&](auto i, auto j, auto small) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < kKeyTiles; ++t) {
+              floatx16 &to = small ? lows[t] : dots[t];
+              to = Mfma32<E>(k[t][i], q[st][j], to);
+            }
+          });
+        } else {
+#pragma unroll
+          for (int t = 0; t < kKeyTiles; ++t) dots[t] = Mfma32<E>(k[t][0], q[st][0], dots[t]);
         }
       }
       if constexpr (kAhead) ReadAhead<4, 1, kKeyTiles * kSteps>();
@@ -589,33 +604,44 @@ __global__ __launch_bounds__(256, WAVES) void AttentionRowsKernel(const Attentio
           weights[n][0] = Pack8<E>(s + n * 8);
         }
       }
+      auto read_v = [&](int n, int c, int p) __attribute__((always_inline)) {
+        const int at = (n * 16 + v_key) * DP + ((c * 4 + v_group) ^ v_swizzle) * 8 + lane % 2 * 4;
+        uint16_t *const from16 = const_cast<uint16_t *>(v_tile) + p * Shape::kPlane + at;
+        typedef __attribute__((address_space(3))) shortx4 *Lds;
+        const uint64_t first = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from16)));
+        const uint64_t second = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from16 + 8 * DP)));
+        return u32x4{static_cast<uint32_t>(first), static_cast<uint32_t>(first >> 32), static_cast<uint32_t>(second), static_cast<uint32_t>(second >> 32)};
+      };
+      if constexpr (kParted) {
 #pragma unroll
-      for (int c = 0; c < kColumns; ++c) {
-        floatx16 low;
+        for (int c0 = 0; c0 < kColumns; c0 += 2) {  // two at a time
+          floatx16 low[2];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) low[e] = 0.0f;
+          for (int e = 0; e < 16; ++e) low[0][e] = 0.0f, low[1][e] = 0.0f;
+#pragma unroll
+          for (int n = 0; n < kKeyTiles * 2; ++n) {
+            u32x4 v[2][kParts];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+              for (int p = 0; p < kParts; ++p) v[c][p] = read_v(n, c0 + c, p);
+            }
+            ForParts([&](auto i, auto j, auto small) __attribute__((always_inline)) {
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                floatx16 &to = small ? low[c] : acc[c0 + c];
+                to = Mfma32<E>(v[c][i], weights[n][j], to);
+              }
+            });
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[c0][e] += low[0][e], acc[c0 + 1][e] += low[1][e];
+        }
+      } else {
 #pragma unroll
         for (int n = 0; n < kKeyTiles * 2; ++n) {
-          u32x4 v[kParts];
 #pragma unroll
-          for (int p = 0; p < kParts; ++p) {
-            const int at = (n * 16 + v_key) * DP + ((c * 4 + v_group) ^ v_swizzle) * 8 + lane % 2 * 4;
-            uint16_t *const from16 = const_cast<uint16_t *>(v_tile) + p * Shape::kPlane + at;
-            typedef __attribute__((address_space(3))) shortx4 *Lds;
-            const shortx4 first = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from16));
-            const shortx4 second = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from16 + 8 * DP));
-            const uint64_t both[2] = {__builtin_bit_cast(uint64_t, first), __builtin_bit_cast(uint64_t, second)};
-            v[p] = u32x4{static_cast<uint32_t>(both[0]), static_cast<uint32_t>(both[0] >> 32), static_cast<uint32_t>(both[1]), static_cast<uint32_t>(both[1] >> 32)};
-          }
-          if constexpr (kParted) {
-            MfmaParts<3>(v, weights[n], acc[c], low);
-          } else {
-            acc[c] = Mfma32<E>(v[0], weights[n][0], acc[c]);
-          }
-        }
-        if constexpr (kParted) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[c][e] += low[e];
+          for (int c = 0; c < kColumns; ++c) acc[c] = Mfma32<E>(read_v(n, c, 0), weights[n][0], acc[c]);
         }
       }
       if constexpr (kAhead) ReadAhead<4, 2, kColumns * kKeyTiles * 2>();

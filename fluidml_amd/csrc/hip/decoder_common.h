@@ -3,6 +3,8 @@
 #ifndef FLUIDML_AMD_CSRC_HIP_DECODER_COMMON_H_
 #define FLUIDML_AMD_CSRC_HIP_DECODER_COMMON_H_
 
+#include <type_traits>
+
 #include "fl_common.h"
 
 namespace fl {
@@ -60,6 +62,20 @@ __device__ __forceinline__ void LoadToLds(const void *from, void *to) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void *)to, 16, 0, 0);
 #endif
+}
+
+// body(part of the left operand, part of the right one, whether the product is one of the small ones) for the six products of fl_common.h's
+// MfmaParts, so that several sums can take turns: products of one sum after the other wait for each other.
+template <typename F>
+__device__ __forceinline__ void ForParts(F &&body) {
+  using std::integral_constant;
+  using Small = std::true_type;
+  body(integral_constant<int, 2>{}, integral_constant<int, 0>{}, Small{});
+  body(integral_constant<int, 0>{}, integral_constant<int, 2>{}, Small{});
+  body(integral_constant<int, 1>{}, integral_constant<int, 1>{}, Small{});
+  body(integral_constant<int, 1>{}, integral_constant<int, 0>{}, Small{});
+  body(integral_constant<int, 0>{}, integral_constant<int, 1>{}, Small{});
+  body(integral_constant<int, 0>{}, integral_constant<int, 0>{}, std::false_type{});
 }
 
 // Waits until matrix instructions (of up to 16 passes) have written their results.  The compiler does this where it sees them read in the same basic

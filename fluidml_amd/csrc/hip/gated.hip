@@ -119,12 +119,20 @@ struct TileShape {
   static_assert(kXGroups % kThreads == 0 && kWGroups % kThreads == 0 && BK % (16 * WK) == 0 && (!GATED || BW / WN == 64), "every thread and wave has the same to do");
 };
 
-// group of eight values in the place of group `group` of row `row`: of x and of ROWS weights (BK values a row), of the others (BW values a row)
+// The group of eight values in the place of group `group` of row `row`.  LDS serves 256 bytes at a time: sixteen lanes' 16 bytes of one group of sixteen
+// rows of x and of ROWS weights (BK values a row), 64 bytes of four rows of the others (BW values a row).  Turned by the row's number those
+// fall on different banks, however many rows lie in 256 bytes.
 template <int BK>
 __device__ __forceinline__ int SwizzledLong(int row, int group) {
-  return group ^ (row & (BK / 8 - 1) & 7);
+  constexpr int kGroups = BK / 8;
+  static_assert(kGroups <= 16, "a row is at most 256 bytes");
+  return group ^ (row / (16 / kGroups) & (kGroups - 1));
 }
-__device__ __forceinline__ int SwizzledWide(int row, int group) { return group ^ (2 * row & 6); }
+template <int BW>
+__device__ __forceinline__ int SwizzledWide(int row, int group) {
+  static_assert(BW == 64 || BW % 128 == 0, "half of 256 bytes or whole ones");
+  return group ^ (BW == 64 ? (row / 2 & 1) * 4 : (row & 3) * 4);
+}
 
 template <typename E>
 __device__ __forceinline__ floatx16 Mfma32(u32x4 x, u32x4 y, floatx16 acc) {
@@ -245,7 +253,7 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::WK > 2 ? 3 : 2) void GatedT
       const bool up = GATED && row >= BN;
       w_offset[n] = (static_cast<uint32_t>(min(up ? row - BN : row, a.columns - 1 - n0)) * static_cast<uint32_t>(up ? a.up_strides[1] : a.gate_strides[1]) + group * 8) * kItem;
     } else {
-      const int row = place / (BW / 8), group = SwizzledWide(row, place % (BW / 8));
+      const int row = place / (BW / 8), group = SwizzledWide<BW>(row, place % (BW / 8));
       const bool up = GATED && group >= BN / 8;
       // (columns behind the last: the last group again, whose results are not stored)
       w_offset[n] = (static_cast<uint32_t>(row) * static_cast<uint32_t>(up ? a.up_strides[0] : a.gate_strides[0]) +
@@ -258,7 +266,7 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::WK > 2 ? 3 : 2) void GatedT
     const T *from = gate_tile + (ROWS ? k0 : k0 * a.gate_strides[0]);
     if constexpr (GATED) {
       const int place = (wave * S::kWLoads + n) * kWave + lane;
-      const bool up = ROWS ? (wave * S::kWLoads + n) * kWave / (BK / 8) >= BN : SwizzledWide(place / (BW / 8), place % (BW / 8)) >= BN / 8;
+      const bool up = ROWS ? (wave * S::kWLoads + n) * kWave / (BK / 8) >= BN : SwizzledWide<BW>(place / (BW / 8), place % (BW / 8)) >= BN / 8;
       if (up) from = up_tile + (ROWS ? k0 : k0 * a.up_strides[0]);
     }
     return reinterpret_cast<const char *>(from) + w_offset[n];
@@ -303,7 +311,7 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::WK > 2 ? 3 : 2) void GatedT
       for (int n = 0; n < S::kWLoads; ++n) {
         const int place = (wave * S::kWLoads + n) * kWave + lane;
         const int row = ROWS ? place / (BK / 8) : place / (BW / 8);
-        const int group = ROWS ? SwizzledLong<BK>(row, place % (BK / 8)) : SwizzledWide(row, place % (BW / 8));
+        const int group = ROWS ? SwizzledLong<BK>(row, place % (BK / 8)) : SwizzledWide<BW>(row, place % (BW / 8));
         const bool up = GATED && (ROWS ? row >= BN : group >= BN / 8);
         const int64_t along = up ? a.up_strides[0] : a.gate_strides[0], across = up ? a.up_strides[1] : a.gate_strides[1];
         const T *from = up ? up_tile : gate_tile;
@@ -384,7 +392,7 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::WK > 2 ? 3 : 2) void GatedT
         } else {
           // sixteen lanes read four of the depth by sixteen columns, and each gets one column's four
           const int row = st * 16 + half * 8 + lane % 16 / 4, group = w_column(j) / 8 + lane / 16 % 2 * 2 + lane % 4 / 2;
-          uint16_t *const from = const_cast<uint16_t *>(w_from) + p * S::kWValues + row * BW + SwizzledWide(row, group) * 8 + lane % 2 * 4;
+          uint16_t *const from = const_cast<uint16_t *>(w_from) + p * S::kWValues + row * BW + SwizzledWide<BW>(row, group) * 8 + lane % 2 * 4;
           typedef __attribute__((address_space(3))) shortx4 *Lds;
           const uint64_t first = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from)));
           const uint64_t second = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + 4 * BW)));
@@ -411,15 +419,22 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::WK > 2 ? 3 : 2) void GatedT
         if (step + 1 < kSteps) read(o[(step + 1) % kSets], stage, step + 1);
       }
       const Operands &now = o[step % kSets];
+      if constexpr (kParted) {
+        ForParts([&](auto p, auto q, auto small) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < S::kRowTiles; ++i) {
+          for (int i = 0; i < S::kRowTiles; ++i) {
 #pragma unroll
-        for (int j = 0; j < S::kWTiles; ++j) {
-          if constexpr (kParted) {
-            MfmaParts<3>(now.w[j], now.x[i], acc[i][j], low[i][j]);
-          } else {
-            acc[i][j] = Mfma32<E>(now.w[j][0], now.x[i][0], acc[i][j]);
+            for (int j = 0; j < S::kWTiles; ++j) {
+              floatx16 &to = small ? low[kParted ? i : 0][kParted ? j : 0] : acc[i][j];
+              to = Mfma32<E>(now.w[j][p], now.x[i][q], to);
+            }
           }
+        });
+      } else {
+#pragma unroll
+        for (int i = 0; i < S::kRowTiles; ++i) {
+#pragma unroll
+          for (int j = 0; j < S::kWTiles; ++j) acc[i][j] = Mfma32<E>(now.w[j][0], now.x[i][0], acc[i][j]);
         }
       }
     }
