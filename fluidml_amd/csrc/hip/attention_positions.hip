@@ -343,7 +343,7 @@ __global__ __launch_bounds__(256, WAVES) void AttentionRowsKernel(const Attentio
   using E = std::conditional_t<kParted, __bf16, T>;
   constexpr int kParts = Shape::kParts, kSteps = DP / 16, kColumns = DP / 32, kKeyTiles = BK / 32;
   // operands read ahead of the products: 4096 queries and keys of 32 heads of 128, 330 -> 321 us; at 64 columns the registers cost the third wave
-  // (114 -> 130), at 256 they are not there (472 -> 519)
+  // (114 -> 130), at 256 there are none to spare (16 heads 527 -> 568)
   constexpr bool kAhead = !kParted && (DP == 96 || DP == 128);
   __shared__ alignas(16) uint16_t lds[Shape::kValues];
 
@@ -1092,6 +1092,9 @@ Plan MakePlan(const fl_tensor *q, const fl_tensor *k, const fl_attention_scores 
   return p;
 }
 
+// Key tiles of 64, of 32 where the columns of 64 keys leave no registers for a second operand: 4096 queries and keys of 16 heads of 256 columns in
+// bf16 take 537 us with 64 keys in a tile and 511 with 32, with a window of 1024 keys 283 and 247. The last argument is the waves of a SIMD that the
+// registers are shared out for: what the tile of that width needs without spilling.
 template <typename T>
 int LaunchRows(const AttentionArgs &a, hipStream_t stream) {
   const dim3 grid(a.tiles_div.divisor * a.heads_div.divisor), block(256);
@@ -1111,7 +1114,7 @@ int LaunchRows(const AttentionArgs &a, hipStream_t stream) {
     } else if (a.columns <= 128) {
       FL_LAUNCH((AttentionRowsKernel<T, 128, 64, 2>), grid, block, 0, stream, a);
     } else {
-      FL_LAUNCH((AttentionRowsKernel<T, 256, 64, 1>), grid, block, 0, stream, a);
+      FL_LAUNCH((AttentionRowsKernel<T, 256, 32, 1>), grid, block, 0, stream, a);
     }
   }
   return LaunchStatus();
