@@ -299,3 +299,102 @@ def test_gated_captured(device):
         assert torch.equal(got[0], products) and torch.equal(got[1], out)
         want, bound = oracle.gated(x, gate, up, gb, ub, "silu")
         check(products, want, oracle.rounded(bound, want, torch.bfloat16))
+
+
+MIDDLE = [(500, 200, 1500), (497, 71, 1501), (512, 1032, 1536), (450, 4200, 1500)]  # too few rows for tiles of 128
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("turned", [True, False], ids=["rows", "columns"])
+@pytest.mark.parametrize("M,K,N", MIDDLE)
+def test_gated_middle_tiles(device, dtype, turned, M, K, N):
+    """Tiles of 64 rows, whose waves share the depth, with two matrices and with one."""
+    import torch
+
+    print("[case]", dtype, turned, M, K, N, flush=True)
+    kind = dtype_of(dtype)
+    x, gate, up, gb, ub = make(device, kind, M, K, N, turned, M % 2 == 1)
+    Oc = 2010 + K % 2
+    down = (torch.randn(Oc, N, device=device) * N ** -0.5).to(kind).t()
+    if not turned:
+        down = down.contiguous()
+    bias, addend = torch.randn(Oc, device=device).to(kind), torch.randn(M, Oc, device=device).to(kind)
+    products, out = torch.full((M, N), 7.0, device=device, dtype=kind), torch.full((M, Oc), 7.0, device=device, dtype=kind)
+    names = kernels(lambda stream: call_block(x, gate, up, gb, ub, down, bias, addend, products, out, "silu", stream))
+    tile = "Li64ELi128E" if dtype == "fp32" else "Li64ELi64E"
+    assert len(names) == 2 and all(tile in name for name in names), names
+    products.fill_(7.0), out.fill_(7.0)
+    call_block(x, gate, up, gb, ub, down, bias, addend, products, out, "silu")
+    want, bound = oracle.gated(x, gate, up, gb, ub, "silu")
+    check(products, want, oracle.rounded(bound, want, kind))
+    h, d = products.double().cpu(), down.double().cpu()
+    want = h @ d + bias.double().cpu() + addend.double().cpu()
+    bound = 2.0 ** -24 * (N + 4) * (h.abs() @ d.abs()) + 2.0 ** -24 * 2 * (want.abs() + addend.double().cpu().abs() + bias.double().cpu().abs())
+    check(out, want, oracle.rounded(bound, want, kind))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_gated_middle_tiles_not_finite(device, dtype):
+    import torch
+
+    M, K, N = 500, 136, 1500
+    x, gate, up, _, _ = make(device, dtype_of(dtype), M, K, N, True, False)
+    gate[50, 7], up[3, 1460], x[M - 1, K - 1], x[5, 0], up[0, 9] = float("nan"), float("inf"), float("nan"), -float("inf"), 0.0
+    out = torch.empty(M, N, device=device, dtype=x.dtype)
+    call(x, gate, up, None, None, out, "relu")
+    want, bound = oracle.gated(x, gate, up, None, None, "relu")
+    assert torch.equal(out.isnan().cpu(), want.isnan()) and torch.equal(out.isinf().cpu(), want.isinf())
+    fine = want.isfinite()  # (what is finite here saw finite operands alone, unless an infinite gate was shut: 0 times a finite sum)
+    assert ((out.double().cpu() - want).abs() <= oracle.rounded(torch.nan_to_num(bound, nan=0.0, posinf=0.0), want, x.dtype))[fine].all()
+
+
+@pytest.mark.parametrize("M", [500, 2003])
+def test_gated_tiles_small_and_large_values(device, M):
+    """fp32 operands near both ends of the range, in tiles whose products are made of parts."""
+    import torch
+
+    for by_x, by_w in ((1e-18, 1e-18), (1e18, 1e-18), (1e15, 1e15), (1.0, 1e-30)):
+        x, gate, up, _, _ = make(device, torch.float32, M, 96, 1500, True, False)
+        x, gate = x * by_x, gate * by_w
+        out = torch.empty(M, 1500, device=device)
+        call(x, gate, up, None, None, out, "identity")
+        want, bound = oracle.gated(x, gate, up, None, None, "identity")
+        beyond = want.abs() > torch.finfo(torch.float32).max
+        assert torch.equal(out.double().cpu()[beyond], want.float().double()[beyond])
+        fine = ~beyond
+        # a product of the first sum below the normal numbers may be taken for none, 96 of them, and the other sum multiplies what is lost
+        lost = 2.0 ** -126 * 96 * (1 + (x.double().cpu() @ up.double().cpu()).abs())
+        check(out.cpu()[fine], want[fine], (bound + lost)[fine])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("M", [500, 2003])
+def test_gated_tiles_views(device, dtype, M):
+    """Operands at odd addresses and odd strides, halves of one tensor, rows apart, results in columns, in tiles."""
+    import torch
+
+    kind = dtype_of(dtype)
+    K, N = 264, 1500
+    x, gate, up, gb, ub = make(device, kind, M, K, N, True, True)
+
+    def shifted(t, by):  # the same values `by` values behind an aligned address, rows an odd number of values apart
+        rows, columns = t.shape
+        flat = torch.full((rows * (columns + 3) + by,), float("nan"), device=device, dtype=kind)
+        view = flat[by:].as_strided((rows, columns), (columns + 3, 1))
+        return view.copy_(t)
+
+    spread = torch.zeros(M, 2 * K, device=device, dtype=kind)[:, ::2]
+    spread.copy_(x)
+    wide = torch.cat([gate, up], 1).contiguous()
+    want, bound = oracle.gated(x, gate, up, gb, ub, "gelu")
+    bound = oracle.rounded(bound, want, kind)
+    for name, xx, g, u in [("odd rows", shifted(x, 1), shifted(gate.t(), 3).t(), shifted(up.t(), 1).t()), ("wide", x, wide[:, :N], wide[:, N:]),
+                           ("odd columns", shifted(x, 2), shifted(gate, 1), shifted(up, 5)), ("spread", spread, gate, up),
+                           ("columns first", x.t().contiguous().t(), gate, up), ("two layouts", x, gate, up.contiguous())]:
+        for out in (torch.full((M, N), 7.0, device=device, dtype=kind), torch.full((N, M), 7.0, device=device, dtype=kind).t(),
+                    torch.full((M, N + 7), 7.0, device=device, dtype=kind)[:, :N]):
+            print("[case]", dtype, M, name, tuple(out.stride()), flush=True)
+            call(xx, g, u, gb, ub, out, "gelu")
+            check(out, want, bound)
+            if out.stride(0) == N + 7:
+                assert (out.as_strided((M, 7), (N + 7, 1), N) == 7.0)[:-1].all()
