@@ -18,7 +18,8 @@ struct AttentionArgs {
   const float *slopes;
   const int32_t *prefix_lengths, *query_documents, *key_documents, *query_starts, *query_lengths, *key_lengths;
   int64_t slope_stride, prefix_stride, query_document_strides[2], key_document_strides[2], query_start_stride, query_length_stride, key_length_stride;
-  int32_t batch, heads, kv_heads, group, queries, keys, columns, causal, window;
+  int64_t window;
+  int32_t batch, heads, kv_heads, group, queries, keys, columns, causal;
   int32_t rows;  // of a key head: queries * group
   float scale2;  // |scale|, in powers of two; its sign is Q's
   float sign, cap, cap2, scale_by_cap, scale_by_cap2;
@@ -33,7 +34,7 @@ struct AttentionArgs {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kBlock = 64;         // keys whose documents the ranges cover
 constexpr float kLazy = 8.0f;      // a maximum may be behind by this many powers of two before the sums are scaled
-constexpr int32_t kFarStart = 1 << 30;  // |query_starts| beyond this is this: no extent reaches so far
+constexpr int64_t kFar = 1 << 30;  // distances to queries further from the keys than this are taken as to here: to a softmax they are the same
 
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -49,22 +50,22 @@ __device__ __forceinline__ Sequence SequenceOf(const AttentionArgs &a, int b) {
   Sequence s;
   s.n_keys = a.key_lengths == nullptr ? a.keys : min(max(a.key_lengths[b * a.key_length_stride], 0), a.keys);
   s.n_queries = a.query_lengths == nullptr ? a.queries : min(max(a.query_lengths[b * a.query_length_stride], 0), a.queries);
-  s.start = a.query_starts == nullptr ? s.n_keys - s.n_queries : min(max(a.query_starts[b * a.query_start_stride], -kFarStart), kFarStart);
+  s.start = a.query_starts == nullptr ? s.n_keys - s.n_queries : a.query_starts[b * a.query_start_stride];
   s.prefix = a.prefix_lengths == nullptr ? 0 : min(max(a.prefix_lengths[b * a.prefix_stride], 0), s.n_keys);
   return s;
 }
 
-// The keys [lo, hi) that query i sees beside the prefix.
+// The keys [lo, hi) that query i sees beside the prefix, 0 <= lo, hi <= n_keys.  (Starts may be any 32-bit number and windows any 64-bit one.)
+__device__ __forceinline__ int32_t Within(const Sequence &s, int64_t j) { return static_cast<int32_t>(min(max(j, int64_t{0}), static_cast<int64_t>(s.n_keys))); }
 __device__ __forceinline__ int32_t FirstKey(const AttentionArgs &a, const Sequence &s, int32_t i) {
-  return a.window == 0 ? 0 : max(s.start + i - a.window + 1, 0);
+  return a.window == 0 ? 0 : Within(s, static_cast<int64_t>(s.start) + i - a.window + 1);
 }
 __device__ __forceinline__ int32_t LastKey(const AttentionArgs &a, const Sequence &s, int32_t i) {
-  const int32_t at = s.start + i;
-  int32_t hi = s.n_keys;
+  const int64_t at = static_cast<int64_t>(s.start) + i;
+  int64_t hi = s.n_keys;
   if (a.causal) hi = min(hi, at + 1);
-  // (a window is at most 2^30 wide and a position at most 2^30 + 2^28)
   if (a.window != 0) hi = min(hi, at + a.window);
-  return max(hi, 0);
+  return Within(s, hi);
 }
 
 // The row of a tile that a lane works for: row r of a key head is head r % group of query r / group.
@@ -81,7 +82,7 @@ __device__ __forceinline__ Row RowOf(const AttentionArgs &a, const Sequence &s, 
   row.head = kv * a.group + (r - row.i * a.group);
   row.there = row.i < s.n_queries;
   const int32_t i = min(row.i, a.queries - 1);  // (what is read for rows that are not there)
-  row.at = s.start + row.i;
+  row.at = static_cast<int32_t>(min(max(static_cast<int64_t>(s.start) + row.i, -kFar), kFar));
   row.document = a.query_documents == nullptr ? 0 : a.query_documents[b * a.query_document_strides[0] + i * a.query_document_strides[1]];
   const bool sees = row.there && row.document >= 0;
   if (row.document < 0) row.document = -2;
@@ -1015,11 +1016,13 @@ int CheckScores(const fl_tensor *q, const fl_tensor *k, const fl_attention_score
   if (q->shape[3] > FL_ATTENTION_MAX_HEAD) return FL_ERR_UNSUPPORTED;
   if (s == nullptr) return FL_ERR_NULL;
   const int64_t B = q->shape[0];
-  if (!std::isfinite(static_cast<float>(s->scale)) || !std::isfinite(static_cast<float>(s->cap)) || s->cap < 0.0) return FL_ERR_ATTR;
+  // (what the kernels multiply by is finite: both by log2(e), and their quotient by twice that)
+  if (!(1.45 * std::fabs(s->scale) < 3e38) || !(2.9 * s->cap < 3e38) || s->cap < 0.0) return FL_ERR_ATTR;
   if (s->cap > 0.0 && !(2.9 * std::fabs(s->scale) / s->cap < 3e38)) return FL_ERR_ATTR;
   if ((s->causal != 0 && s->causal != 1) || s->window < 0) return FL_ERR_ATTR;
-  // 32-bit counts: rows of a key head, sequences and key heads
-  if (q->shape[2] * (q->shape[1] / k->shape[1]) > (1 << 28) || q->shape[0] * k->shape[1] > (1 << 28) || q->shape[0] > 65535) return FL_ERR_TOO_LARGE;
+  // what a grid of workgroups counts: tiles of rows of all key heads, sequences
+  const __int128 tiles = (q->shape[2] * (q->shape[1] / k->shape[1]) + 15) / 16;
+  if (tiles * q->shape[0] * k->shape[1] > kMostWorkgroups - 1536 || q->shape[0] > 65535) return FL_ERR_TOO_LARGE;
   FL_CHECK(CheckOptionalVector(s->slopes, FL_FLOAT32, q->shape[1]));
   FL_CHECK(CheckLengths(s->prefix_lengths, B));
   FL_CHECK(CheckLengths(s->query_starts, B));
@@ -1073,7 +1076,7 @@ Plan MakePlan(const fl_tensor *q, const fl_tensor *k, const fl_attention_scores 
   if (!p.many) {
     const int64_t tiles = B * KV * ((rows + 15) / 16);
     int64_t reach = Skv;
-    if (s->window > 0 && s->prefix_lengths == nullptr) reach = std::min(reach, s->window * (s->causal ? 1 : 2) + 16);
+    if (s->window > 0 && s->prefix_lengths == nullptr) reach = std::min(reach, std::min(s->window, Skv) * (s->causal ? 1 : 2) + 16);
     const int64_t keys = q->dtype == FL_FLOAT32 ? 16 : 32;
     int64_t splits = std::min<int64_t>((1536 + tiles - 1) / tiles, reach / (4 * 2 * keys));
     splits = std::min(splits, kPartialBytes / (B * KV * rows * (D + 2) * 4));
@@ -1182,8 +1185,7 @@ int fluidml_hip_attention_positions(const fl_tensor *q, const fl_tensor *k, cons
   a.columns = static_cast<int32_t>(q->shape[3]);
   a.rows = a.queries * a.group;
   a.causal = scores->causal;
-  // (no two positions are further apart than this, so a wider window is none)
-  a.window = static_cast<int32_t>(std::min<int64_t>(scores->window, INT32_C(0x5fffffff)));
+  a.window = std::min<int64_t>(scores->window, INT64_C(1) << 33);  // (no two positions are further apart)
   a.sign = scores->scale < 0.0 ? -1.0f : 1.0f;
   const double scale = std::fabs(scores->scale), log2e = 1.4426950408889634;
   a.scale2 = static_cast<float>(scale * log2e);
@@ -1199,7 +1201,6 @@ int fluidml_hip_attention_positions(const fl_tensor *q, const fl_tensor *k, cons
   for (int i = 0; i < 3; ++i) a.out_aligned = a.out_aligned && (out->shape[i] == 1 || out->strides[i] % 4 == 0);
   const uint32_t heads = static_cast<uint32_t>(a.batch) * static_cast<uint32_t>(a.kv_heads);
   const uint32_t tiles = static_cast<uint32_t>(plan.many ? (a.rows + 127) / 128 : (a.rows + 15) / 16);
-  if (static_cast<int64_t>(heads) * tiles * plan.splits > INT32_MAX) return FL_ERR_TOO_LARGE;
   a.by_xcd = heads % 8 == 0;
   a.group_div = FastDiv(static_cast<uint32_t>(a.group));
   a.kv_div = FastDiv(static_cast<uint32_t>(a.kv_heads));

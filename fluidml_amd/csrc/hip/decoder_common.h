@@ -9,6 +9,9 @@
 
 namespace fl {
 
+// of 256 threads: a grid has fewer than 2^32 threads
+constexpr int64_t kMostWorkgroups = (INT64_C(1) << 24) - 1;
+
 inline bool IsDecoderType(int32_t dtype) { return dtype == FL_FLOAT32 || dtype == FL_FLOAT16 || dtype == FL_BFLOAT16; }
 
 // CheckView for these operators: 64-bit offsets, FL_BFLOAT16 among the types

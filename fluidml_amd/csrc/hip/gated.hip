@@ -816,6 +816,9 @@ int CheckMatrix(const fl_tensor *t, int32_t dtype, int64_t rows, int64_t columns
   return t->shape[0] == rows && t->shape[1] == columns ? FL_OK : FL_ERR_SHAPE;
 }
 
+// a result that any of the kernels' grids counts: its tiles have 16 columns or more, 8192 places or more where there are many
+int CheckExtents(int64_t rows, int64_t columns) { return columns > (1 << 26) || rows * columns > (INT64_C(1) << 36) ? FL_ERR_TOO_LARGE : FL_OK; }
+
 int CheckGated(const fl_tensor *x, const fl_tensor *gate, const fl_tensor *up, const fl_tensor *gate_bias, const fl_tensor *up_bias,
                const fl_tensor *products, int32_t activation) {
   FL_CHECK(CheckWideView(x));
@@ -829,7 +832,7 @@ int CheckGated(const fl_tensor *x, const fl_tensor *gate, const fl_tensor *up, c
   FL_CHECK(CheckOptionalVector(gate_bias, x->dtype, N));
   FL_CHECK(CheckOptionalVector(up_bias, x->dtype, N));
   if (activation < FL_GATE_SILU || activation > FL_GATE_IDENTITY) return FL_ERR_ATTR;
-  return FL_OK;
+  return CheckExtents(M, N);
 }
 
 void Set(const fl_tensor *t, int64_t (&strides)[2]) {
@@ -844,7 +847,6 @@ int Run(const fl_tensor *t, int unit) {
 template <typename T, typename Shape>
 int LaunchTiles(GatedArgs &a, hipStream_t stream) {
   const int64_t rows = (a.rows + Shape::BM - 1) / Shape::BM, columns = (a.columns + Shape::BN - 1) / Shape::BN;
-  if (rows * columns > INT32_MAX / 16) return FL_ERR_TOO_LARGE;
   a.row_tiles = FastDiv(static_cast<uint32_t>(rows));
   a.column_tiles = FastDiv(static_cast<uint32_t>(columns));
   a.group = FastDiv(static_cast<uint32_t>(std::min<int64_t>(rows, 8) * columns));
@@ -855,7 +857,6 @@ int LaunchTiles(GatedArgs &a, hipStream_t stream) {
 template <typename T, typename Shape>
 int LaunchFew(GatedArgs &a, hipStream_t stream) {
   const int64_t rows = (a.rows + Shape::RT * 16 - 1) / (Shape::RT * 16), columns = (a.columns + Shape::kColumns - 1) / Shape::kColumns;
-  if (rows * columns > INT32_MAX / 16) return FL_ERR_TOO_LARGE;
   a.row_tiles = FastDiv(static_cast<uint32_t>(rows));
   a.column_tiles = FastDiv(static_cast<uint32_t>(columns));
   FL_LAUNCH((GatedFewKernel<T, Shape>), dim3(static_cast<uint32_t>(rows * columns)), dim3(512), 0, stream, a);
@@ -938,6 +939,7 @@ int fluidml_hip_gated_feed_forward(const fl_tensor *x, const fl_tensor *gate, co
   FL_CHECK(CheckMatrix(out, x->dtype, M, O, true));
   FL_CHECK(CheckOptionalVector(down_bias, x->dtype, O));
   if (addend != nullptr) FL_CHECK(CheckMatrix(addend, x->dtype, M, O));
+  FL_CHECK(CheckExtents(M, O));
   FL_CHECK(Contract(x, gate, up, gate_bias, up_bias, nullptr, products, activation, AsStream(stream)));
   return Contract(products, down, nullptr, down_bias, nullptr, addend, out, FL_GATE_IDENTITY, AsStream(stream));
 }

@@ -163,7 +163,7 @@ int CheckPlan(const fl_rotary_plan *p, int64_t columns) {
   if (p->interleaved != 0 && p->interleaved != 1) return FL_ERR_ATTR;
   if (p->dims < 2 || p->dims % 2 != 0 || p->dims > columns) return FL_ERR_ATTR;
   if (p->dims > FL_ROTARY_MAX_DIMS) return FL_ERR_UNSUPPORTED;
-  if (!(p->base > 1.0) || !std::isfinite(p->base) || !std::isfinite(p->amplitude)) return FL_ERR_ATTR;
+  if (!(p->base > 1.0) || !std::isfinite(p->base) || !std::isfinite(static_cast<float>(p->amplitude))) return FL_ERR_ATTR;
   if (p->scaling < FL_ROTARY_PLAIN || p->scaling > FL_ROTARY_DIMENSION) return FL_ERR_ATTR;
   if (p->scaling != FL_ROTARY_PLAIN && (!(p->factor >= 1.0) || !std::isfinite(p->factor))) return FL_ERR_ATTR;
   if (p->scaling == FL_ROTARY_WAVELENGTH || p->scaling == FL_ROTARY_DIMENSION) {
@@ -267,6 +267,7 @@ int Rotate(int n, const fl_tensor *const *x, const fl_tensor *const *out, const 
   }
   a.amplitude = static_cast<float>(plan->amplitude);
 
+  if ((B * S + group - 1) / group > kMostWorkgroups) return FL_ERR_TOO_LARGE;
   const dim3 grid(static_cast<uint32_t>((B * S + group - 1) / group));
   FL_CHECK(ForDecoderType(x[0]->dtype, [&](auto type) {
     using T = decltype(type);

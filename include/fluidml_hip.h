@@ -628,6 +628,11 @@ int fluidml_hip_add_layer_normalization(const fl_tensor *lhs, const fl_tensor *r
 /* the current device, which is the stream's.  The calls allocate nothing,     */
 /* synchronise nothing and may be captured; two calls that may run at the same */
 /* time (a replayed graph among them) need scratch and results of their own.   */
+/* FL_ERR_TOO_LARGE, nothing launched: more than a grid counts, which is       */
+/* attention of 2^28 rows (B H Sq; less where H / KV Sq is below 16) or of     */
+/* more than 65535 sequences, a result of the gated block of more than 2^36    */
+/* values or 2^26 columns, rotary positions of some 2^24 tokens whose heads    */
+/* are a workgroup's work each.                                                */
 #define FL_DECODER_MAX_EXTENT (1 << 28)
 
 /* Rotary positions.  The pair j < dims / 2 of columns (a, b) of a token at position p becomes
@@ -651,7 +656,7 @@ typedef struct fl_rotary_plan {
   double factor;       /* >= 1; what a scaling does not use is not looked at */
   double original_length; /* > 0 */
   double low, high;       /* 0 < low < high */
-  double amplitude;       /* finite; 1 where nothing else is wanted */
+  double amplitude;       /* finite in 32 bits; 1 where nothing else is wanted */
 } fl_rotary_plan;
 /* x, out [B, H, S, D], any strides; `out` may be `x` itself.  positions: int32 or int64, [S], [1, S] or [B, S], of either sign. */
 int fluidml_hip_rotary_positions(const fl_tensor *x, const fl_tensor *positions, const fl_tensor *out, const fl_rotary_plan *plan, void *stream);
@@ -661,7 +666,7 @@ int fluidml_hip_rotary_positions_pair(const fl_tensor *x0, const fl_tensor *out0
 /* Attention whose scores and masks go by positions, so that no mask is read and keys that no query of a tile sees cost
  * nothing:
  *   s_ij = scale (q_i . k_j);  cap > 0: s_ij = cap tanh(s_ij / cap);  slopes: s_ij -= slopes[h] |p_i - j|
- *   out_i = sum_j softmax_j(s_ij) v_j over the keys that query i sees; zeros where it sees none
+ *   out_i = sum_j softmax_j(s_ij) v_j over the keys that query i sees; zeros where it sees none (or none above minus infinity)
  * q, out [B, H, Sq, D], k, v [B, KV, Skv, D], any strides; head h reads key head h / (H / KV) (H a multiple of KV); D <=
  * FL_ATTENTION_MAX_HEAD.  Key j of a sequence is at position j, query i at p_i = query_starts[b] + i, without query_starts
  * at key_lengths[b] - query_lengths[b] + i (the last query at the last key).  Query i sees key j where all of these hold:

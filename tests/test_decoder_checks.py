@@ -128,3 +128,34 @@ def test_gated_refusals(cabi):
         t[i] = None
         assert cabi.lib.fluidml_hip_gated_matmul(*t, 0, None) == NULL
     assert rc(x=(0, 8)) == SHAPE
+
+
+def test_extents_beyond_a_grid(cabi):
+    """What no grid counts is refused before anything is launched, and no size is computed that 64 bits do not hold.  (Views of overlapping
+    places: nothing is read.)"""
+    lib, size = cabi.lib, ctypes.c_size_t()
+    scores = cabi.FlAttentionScores(1.0)
+    # (the fourth: tiles of one row each; with one key head its 2^24 rows would be 2^20 tiles of sixteen, which a grid counts)
+    for B, H, KV, S, D in ((1, 1 << 28, 1, 1 << 28, 254), (1, 1 << 28, 1 << 28, 1 << 28, 254), (1 << 16, 1 << 12, 1, 1 << 28, 2), (1, 1 << 24, 1 << 24, 1, 8),
+                           (65536, 1, 1, 1, 8), (1, 1, 1, 1 << 28, 8)):
+        q, k = tensor(cabi, B, H, S, D, strides=(1, 1, 1, 1)), tensor(cabi, B, KV, 9, D, strides=(1, 1, 1, 1))
+        assert lib.fluidml_hip_attention_positions_scratch(p(q), p(k), p(scores), p(size)) == LARGE
+        assert lib.fluidml_hip_attention_positions(p(q), p(k), p(k), p(q), p(scores), None, 0, None) == LARGE
+    x, w, o = tensor(cabi, 1, 8), tensor(cabi, 8, 1 << 27), tensor(cabi, 1, 1 << 27)
+    assert lib.fluidml_hip_gated_matmul(p(x), p(w), p(w), None, None, p(o), 0, None) == LARGE
+    x, w, o = tensor(cabi, 1 << 28, 8), tensor(cabi, 8, 512), tensor(cabi, 1 << 28, 512)
+    assert lib.fluidml_hip_gated_matmul(p(x), p(w), p(w), None, None, p(o), 0, None) == LARGE
+    x, w, down, small, o = tensor(cabi, 1 << 28, 8), tensor(cabi, 8, 16), tensor(cabi, 16, 512), tensor(cabi, 1 << 28, 16), tensor(cabi, 1 << 28, 512)
+    assert lib.fluidml_hip_gated_feed_forward(p(x), p(w), p(w), None, None, p(down), None, None, p(small), p(o), 0, None) == LARGE
+    plan = cabi.FlRotaryPlan(0, 0, 8, 1e4, 1, 1, 1, 4, 1)
+    x, i = tensor(cabi, 1 << 12, 4096, 1 << 13, 8), tensor(cabi, 1 << 13, dtype=cabi.FL_INT32)
+    assert lib.fluidml_hip_rotary_positions(p(x), p(i), p(x), p(plan), None) == LARGE
+
+
+def test_factors_beyond_32_bits(cabi):
+    q, k = tensor(cabi, 2, 4, 5, 64), tensor(cabi, 2, 2, 9, 64)
+    for scale, cap in ((3e38, 0.0), (-3e38, 0.0), (1.0, 3e38), (1.0, 1e300), (1e30, 1e-30)):
+        scores = cabi.FlAttentionScores(scale, cap)
+        assert cabi.lib.fluidml_hip_attention_positions(p(q), p(k), p(k), p(q), p(scores), None, 0, None) == ATTR, (scale, cap)
+    x, i, plan = tensor(cabi, 1, 1, 1, 8), tensor(cabi, 1, dtype=cabi.FL_INT32), cabi.FlRotaryPlan(0, 0, 8, 1e4, 1, 1, 1, 4, 1e39)
+    assert cabi.lib.fluidml_hip_rotary_positions(p(x), p(i), p(x), p(plan), None) == ATTR

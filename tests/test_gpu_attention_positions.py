@@ -334,3 +334,43 @@ def test_attention_positions_captured(device):
         oracle.call_attention(q, k, v, out, 0.1, **more)
         torch.cuda.synchronize()
         assert torch.equal(out, got)  # the same bits, every time
+
+
+@pytest.mark.parametrize("B,H,KV,Sq,Skv", [(6, 2, 1, 3, 200), (6, 32, 32, 130, 90)], ids=["few", "many"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_attention_positions_far_starts(device, dtype, B, H, KV, Sq, Skv):
+    """Starts up to the ends of 32 bits with windows that reach as far and windows of any 64-bit width, and biases of such distances."""
+    import torch
+
+    q, k, v = draw(device, dtype_of(dtype), (B, H, Sq, 64), (B, KV, Skv, 64), (B, KV, Skv, 64))
+    starts = torch.tensor([2 ** 31 - 1, -2 ** 31, 2 ** 30 - 1, 40, 1 - 2 ** 30, -Sq], dtype=torch.int32, device=device)
+    for causal in (True, False):
+        for window in (0, 7, 2 ** 30, 2 ** 30 + 5, 2 ** 31 - 1, 2 ** 31 + 50, 2 ** 62):
+            print("[case]", dtype, causal, window, flush=True)
+            out = torch.full_like(q, 7.0)
+            oracle.call_attention(q, k, v, out, 0.125, causal=causal, window=window, starts=starts)
+            check(q, k, v, out, 0.125, causal=causal, window=window, starts=starts)
+    # a bias of a far query is one number for all its keys: small slopes, so that its roundings (2^-24 of it) stay below the scores
+    slopes = 2.0 ** -(24 + torch.arange(H, device=device, dtype=torch.float32) % 4)
+    out = torch.full_like(q, 7.0)
+    near = starts.clamp(-2 ** 24, 2 ** 24)
+    oracle.call_attention(q, k, v, out, 0.125, slopes=slopes, starts=near)
+    check(q, k, v, out, 0.125, slopes=slopes, starts=near)
+
+
+def test_attention_positions_many_rows_large_offsets(device):
+    """Keys and values beyond 2^31 elements where a workgroup has 128 rows: steps that 32 bits hold and steps that they do not."""
+    import torch
+
+    D, H, Sq = 64, 12, 2100
+    pool = torch.zeros(2 ** 31 + (1 << 24), dtype=torch.bfloat16, device=device)
+    for T in (70, 300):
+        stride = (2 ** 31) // (T - 1) // 8 * 8
+        k, v = (pool.as_strided((1, 1, T, D), (0, 0, stride, 1), at) for at in (0, 4096))
+        q, kk, vv = draw(device, torch.bfloat16, (1, H, Sq, D), (1, 1, T, D), (1, 1, T, D))
+        k.copy_(kk)
+        v.copy_(vv)
+        out = torch.empty_like(q)
+        assert any("AttentionRowsKernel" in name for name in kernels(q, k, v, out, 0.125))
+        oracle.call_attention(q, k, v, out, 0.125)
+        check(q, kk, vv, out, 0.125)
