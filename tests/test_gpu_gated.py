@@ -398,3 +398,22 @@ def test_gated_tiles_views(device, dtype, M):
             check(out, want, bound)
             if out.stride(0) == N + 7:
                 assert (out.as_strided((M, 7), (N + 7, 1), N) == 7.0)[:-1].all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("turned", [True, False], ids=["rows", "columns"])
+@pytest.mark.parametrize("M,K,N", [(500, 1, 1500), (500, 5, 1500), (2003, 7, 1100), (20001, 40, 3), (33000, 71, 1), (20000, 3, 5)])
+def test_gated_tiles_thin(device, dtype, turned, M, K, N):
+    """A depth or columns below one load's values, in tiles."""
+    import torch
+
+    print("[case]", dtype, turned, M, K, N, flush=True)
+    kind = dtype_of(dtype)
+    x, gate, up, gb, ub = make(device, kind, M, K, N, turned, True)
+    out = torch.full((M, N), 7.0, device=device, dtype=kind)
+    name, = kernels(lambda stream: call(x, gate, up, gb, ub, out, "silu", stream))
+    assert "GatedTileKernel" in name
+    out.fill_(7.0)
+    call(x, gate, up, gb, ub, out, "silu")
+    want, bound = oracle.gated(x, gate, up, gb, ub, "silu")
+    check(out, want, oracle.rounded(bound, want, kind))
