@@ -970,9 +970,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void AttentionFewKernel(con
   }
 }
 
-// Joins the splits, a wave a row.
-template <typename T>
+// Joins the splits, a wave a row, in their order.  What counts is how many loads are on their way: those of kRun splits at a time (32 rows of 128
+// columns in 64 splits: one at a time 23.5 us, sixteen 5.1).
+template <typename T, int DP>
 __global__ __launch_bounds__(256) void AttentionJoinKernel(const AttentionArgs a) {
+  constexpr int kColumns = DP / kWave, kRun = 16;
   const int lane = threadIdx.x % kWave;
   const int64_t all_rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.rows;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -981,22 +983,32 @@ __global__ __launch_bounds__(256) void AttentionJoinKernel(const AttentionArgs a
   const int32_t r = static_cast<int32_t>(at - static_cast<int64_t>(head) * a.rows);
   const int b = static_cast<int>(a.kv_div.Div(head)), kv = static_cast<int>(head) - b * a.kv_heads;
   if (static_cast<int32_t>(a.group_div.Div(r)) >= SequenceOf(a, b).n_queries) return;
-  float higher = -INFINITY, total = 0.0f, x[FL_ATTENTION_MAX_HEAD / kWave] = {};
   // (at most 64 splits: a lane reads the figures of one)
   const float2 own = lane < a.splits ? a.stats[lane * all_rows + at] : make_float2(-INFINITY, 0.0f);
-  higher = WaveReduce(own.x, MaxOp{});
+  const float higher = WaveReduce(own.x, MaxOp{});
   const float kept = __builtin_amdgcn_exp2f(own.x - (higher == -INFINITY ? 0.0f : higher));
-  total = GroupSum<64>(own.y * kept);
-  for (int s = 0; s < a.splits; ++s) {
-    const float by = __shfl(kept, s);
-    const float *const from = a.partial + (s * all_rows + at) * a.columns;
+  const float total = GroupSum<64>(own.y * kept);
+  float x[FL_ATTENTION_MAX_HEAD / kWave] = {};
+  for (int s0 = 0; s0 < a.splits; s0 += kRun) {
+    float part[kRun][kColumns];
 #pragma unroll
-    for (int c = 0; c < FL_ATTENTION_MAX_HEAD / kWave; ++c) {
-      if (c * kWave + lane < a.columns) x[c] += from[c * kWave + lane] * by;
+    for (int n = 0; n < kRun; ++n) {  // (no branch around a load: splits and columns that are not there are the last ones again)
+      const float *const from = a.partial + (min(s0 + n, a.splits - 1) * all_rows + at) * a.columns;
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c) part[n][c] = from[min(c * kWave + lane, a.columns - 1)];
+    }
+#pragma unroll
+    for (int n = 0; n < kRun; ++n) {
+      const float by = __shfl(kept, min(s0 + n, a.splits - 1));
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c) x[c] = s0 + n < a.splits ? x[c] + part[n][c] * by : x[c];
     }
   }
   StoreRow<T>(a, b, kv, r, x, total);
 }
+
+constexpr int64_t kPartialBytes = 16 << 20;  // of the splits' sums
+constexpr int64_t kSplitWorkgroups = 768;
 
 int CheckLengths(const fl_tensor *t, int64_t batch) { return CheckOptionalVector(t, FL_INT32, batch); }
 
@@ -1022,7 +1034,7 @@ int CheckScores(const fl_tensor *q, const fl_tensor *k, const fl_attention_score
   if ((s->causal != 0 && s->causal != 1) || s->window < 0) return FL_ERR_ATTR;
   // what a grid of workgroups counts: tiles of rows of all key heads, sequences
   const __int128 tiles = (q->shape[2] * (q->shape[1] / k->shape[1]) + 15) / 16;
-  if (tiles * q->shape[0] * k->shape[1] > kMostWorkgroups - 1536 || q->shape[0] > 65535) return FL_ERR_TOO_LARGE;
+  if (tiles * q->shape[0] * k->shape[1] > kMostWorkgroups - kSplitWorkgroups || q->shape[0] > 65535) return FL_ERR_TOO_LARGE;
   FL_CHECK(CheckOptionalVector(s->slopes, FL_FLOAT32, q->shape[1]));
   FL_CHECK(CheckLengths(s->prefix_lengths, B));
   FL_CHECK(CheckLengths(s->query_starts, B));
@@ -1065,20 +1077,23 @@ bool Aligned(const fl_tensor *t) {
   return true;
 }
 
-constexpr int64_t kPartialBytes = 16 << 20;
-
 // (of K and V only the extents and K's alignment are known here; `aligned`: that of both)
 Plan MakePlan(const fl_tensor *q, const fl_tensor *k, const fl_attention_scores *s, bool aligned) {
   const int64_t B = q->shape[0], KV = k->shape[1], Skv = k->shape[2], D = q->shape[3], rows = q->shape[2] * (q->shape[1] / KV);
   Plan p{};
-  p.many = aligned && rows > 32 && B * KV * ((rows + 127) / 128) >= 192;
+  // Tiles of 128 rows where there are enough of them to fill the chip, else of 16 whose keys are split.  32 heads of 128 columns in bf16, 4096 keys:
+  // 96 tiles of 128 rows 112 us (split tiles of 16: 145), 64 tiles 111 (111), 32 tiles 110 (72); in fp32, 64 columns, 128 tiles 36 (52), 48 tiles
+  // 217 (102).  Up to 32 rows of a key head most of 128 would be empty: 115 us where tiles of 128 take 264.
+  p.many = aligned && rows > 32 && B * KV * ((rows + 127) / 128) >= 96;
   p.splits = 1;
   if (!p.many) {
     const int64_t tiles = B * KV * ((rows + 15) / 16);
     int64_t reach = Skv;
     if (s->window > 0 && s->prefix_lengths == nullptr) reach = std::min(reach, std::min(s->window, Skv) * (s->causal ? 1 : 2) + 16);
     const int64_t keys = q->dtype == FL_FLOAT32 ? 16 : 32;
-    int64_t splits = std::min<int64_t>((1536 + tiles - 1) / tiles, reach / (4 * 2 * keys));
+    // three workgroups for each compute unit, each wave with two tiles of keys or more: 8 sequences of 8 key heads, 8192 keys, 12 splits 53.0 us and
+    // 5.1 to join them, 24 splits 52.8 and 5.8, 48 splits 58 and more; 16 heads of fp32, 128 queries, 39 and 4.8 with 6 splits, 44 and 4.7 with 12
+    int64_t splits = std::min<int64_t>((kSplitWorkgroups + tiles - 1) / tiles, reach / (4 * 2 * keys));
     splits = std::min(splits, kPartialBytes / (B * KV * rows * (D + 2) * 4));
     p.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(splits, 64)));
   }
@@ -1134,7 +1149,7 @@ int LaunchFew(const AttentionArgs &a, bool aligned, hipStream_t stream) {
   FL_CHECK(LaunchStatus());
   if (a.splits > 1) {
     const int64_t rows = static_cast<int64_t>(a.heads_div.divisor) * a.rows;
-    FL_LAUNCH(AttentionJoinKernel<T>, dim3(static_cast<uint32_t>((rows + 3) / 4)), block, 0, stream, a);
+    FL_LAUNCH((AttentionJoinKernel<T, DP>), dim3(static_cast<uint32_t>((rows + 3) / 4)), block, 0, stream, a);
   }
   return LaunchStatus();
 }

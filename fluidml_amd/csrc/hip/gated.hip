@@ -863,6 +863,11 @@ int LaunchFew(GatedArgs &a, hipStream_t stream) {
   return LaunchStatus();
 }
 
+// The largest tiles that still fill the chip.  Gated, weights as [N, K], in us (other choice):
+//   16-bit, depth 4096: 256 x 256 in 208 tiles 125 (128 x 128: 152), in 160 tiles 125 (130); 128 x 128 in 128 tiles 57 (64 x 64: 57), in 96 tiles 53
+//   (55); 64 x 64 in 256 tiles 50 (32 rows, few: 66), in 128 tiles 40 (33)
+//   fp32, depth 1024: 128 x 128 in 256 tiles 75 (64 x 128: 76), in 128 tiles 69 (39); 64 x 128 in 128 tiles 35 (few: 43), in 64 tiles 34 (23)
+//   few rows: 32 of them in 512 workgroups 33 (16: 47), in 128 workgroups 17.6 (13.7)
 template <typename T, bool GATED, bool ROWS>
 int LaunchLayout(GatedArgs &a, hipStream_t stream) {
   auto tiles = [&](int64_t bm, int64_t bw) { return (a.rows + bm - 1) / bm * ((a.columns + bw / (GATED ? 2 : 1) - 1) / (bw / (GATED ? 2 : 1))); };
@@ -872,7 +877,7 @@ int LaunchLayout(GatedArgs &a, hipStream_t stream) {
     if (tiles(128, 128) >= 256) return LaunchTiles<T, TileShape<T, 128, 128, 2, 2, 1, 32, GATED, ROWS>>(a, stream);
     if (tiles(64, 128) >= 128) return LaunchTiles<T, TileShape<T, 64, 128, 2, 2, 2, 64, GATED, ROWS>>(a, stream);
   } else {
-    if (tiles(256, 256) >= 200 && a.x_direct && a.weights_direct && a.depth % 64 == 0) return LaunchTiles<T, TileShape<T, 256, 256, 2, 4, 1, 64, GATED, ROWS>>(a, stream);
+    if (tiles(256, 256) >= 160 && a.x_direct && a.weights_direct && a.depth % 64 == 0) return LaunchTiles<T, TileShape<T, 256, 256, 2, 4, 1, 64, GATED, ROWS>>(a, stream);
     if (tiles(128, 128) >= 128) return LaunchTiles<T, TileShape<T, 128, 128, 2, 2, 1, 64, GATED, ROWS>>(a, stream);
     if (tiles(64, 64) >= 256) return LaunchTiles<T, TileShape<T, 64, 64, 1, 1, 4, 64, GATED, ROWS>>(a, stream);
   }
