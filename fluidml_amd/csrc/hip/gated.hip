@@ -101,6 +101,8 @@ __device__ __forceinline__ float CarefulDot(const GatedArgs &a, const void *weig
 // which is split into three bf16 parts on the way) through registers, zeros behind the ends.
 // Weights lie in LDS as they lie in memory, a row for each column of the product (ROWS: a checkpoint's [N, K]) or a row for each of the
 // depth ([K, N], turned by the transposing read).  Groups of 16 bytes are permuted within a row against bank conflicts.
+// bf16, 8192 rows of 4096, 14336 columns: 1650 us gated (1166 TFLOP/s), 800 us back (1202); a library's plain product of that kind reaches 1378, at
+// which both would take 2094.  Bound by the matrix pipe and the power it leaves the clock.  fp32 in three parts: 4096^3 165 TFLOP/s.
 template <typename T, int BM_, int BW_, int WM_, int WN_, int WK_, int BK_, bool GATED_, bool ROWS_>
 struct TileShape {
   static constexpr int BM = BM_, BW = BW_, WM = WM_, WN = WN_, WK = WK_, BK = BK_;
@@ -603,6 +605,7 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::WK > 2 ? 3 : 2) void GatedT
 // its way while one is multiplied.
 // ROWS: a lane loads 16 bytes of the depth of column lane % 16.  Otherwise four columns of each of the depth's values of its quarter of the wave,
 // and turns them around in registers.  fp32 stays fp32: at few rows its products cost less than the bytes.
+// bf16, 4 rows of 4096, 11008 columns: 34 us gated (180 MB, 5.4 TB/s), 19 us back (90 MB, 4.8 TB/s).
 template <typename T, bool GATED_, bool ROWS_, int RT_>
 struct FewShape {
   static constexpr bool GATED = GATED_, ROWS = ROWS_, kWide = std::is_same_v<T, float>;
