@@ -323,12 +323,16 @@ _STRIDES = [struct.Struct(f"={n}q") for n in range(FL_MAX_RANK + 1)]
 
 
 def view(t) -> FlTensor:
-    """The view that a torch tensor is: its address, type, shape and strides (the tensor has to outlive its uses)."""
+    """The view that a torch tensor on a GPU is: its address, type, shape and strides (the tensor has to outlive its uses)."""
+    if not t.is_cuda:
+        raise ValueError(f"a tensor on {t.device}: kernels read and write device memory")
     rank = t.dim()
     if rank > FL_MAX_RANK:
         raise ValueError(f"rank {rank} exceeds FL_MAX_RANK={FL_MAX_RANK}")
     dtype = _DTYPE_OF.get(t.dtype)
     if dtype is None:
+        if str(t.dtype) not in _TORCH_DTYPES:
+            raise ValueError(f"no view of {t.dtype}")
         dtype = _DTYPE_OF[t.dtype] = _TORCH_DTYPES[str(t.dtype)]
     v = FlTensor()
     _HEAD[rank].pack_into(v, 0, t.data_ptr(), dtype, rank, *t.shape)

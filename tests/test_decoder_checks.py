@@ -159,3 +159,26 @@ def test_factors_beyond_32_bits(cabi):
         assert cabi.lib.fluidml_hip_attention_positions(p(q), p(k), p(k), p(q), p(scores), None, 0, None) == ATTR, (scale, cap)
     x, i, plan = tensor(cabi, 1, 1, 1, 8), tensor(cabi, 1, dtype=cabi.FL_INT32), cabi.FlRotaryPlan(0, 0, 8, 1e4, 1, 1, 1, 4, 1e39)
     assert cabi.lib.fluidml_hip_rotary_positions(p(x), p(i), p(x), p(plan), None) == ATTR
+
+
+def test_view_refusals(cabi):
+    """Host memory has no view: a kernel that got its address would fault."""
+    import torch
+
+    for t in (torch.zeros(2, 3), torch.zeros(2, dtype=torch.complex64), torch.zeros(2, device="meta")):
+        with pytest.raises(ValueError):
+            cabi.view(t)
+
+
+@pytest.mark.gpu
+def test_views(cabi, device):
+    import torch
+
+    for dtype, code in ((torch.bfloat16, cabi.FL_BFLOAT16), (torch.float16, cabi.FL_FLOAT16), (torch.float32, cabi.FL_FLOAT32), (torch.int64, cabi.FL_INT64)):
+        t = torch.zeros(5, 7, 3, dtype=dtype, device=device)[1:, ::2].transpose(0, 2)
+        v = cabi.view(t)
+        assert (v.base, v.dtype, v.rank) == (t.data_ptr(), code, 3)
+        assert tuple(v.shape[:3]) == tuple(t.shape) and tuple(v.strides[:3]) == t.stride()
+    for t in (torch.zeros(2, dtype=torch.complex64, device=device), torch.zeros([1] * (cabi.FL_MAX_RANK + 1), device=device)):
+        with pytest.raises(ValueError):
+            cabi.view(t)
